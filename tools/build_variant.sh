@@ -4,7 +4,7 @@
 set -e
 cd "$(dirname "$0")/../mars5-tts_amd/csrc"
 NAME=$1; SRC=$2; EXTRA=$3
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -ffp-contract=off -Wno-unused-result -DM5_TOOLS"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -ffp-contract=off -Wno-unused-result -DM5_TOOLS -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p obj_tools_$NAME
 cp obj_tools/*.o obj_tools_$NAME/
 hipcc $FLAGS $EXTRA -c $SRC.hip -o obj_tools_$NAME/$SRC.o
