@@ -22,6 +22,7 @@
 #ifndef MARS5_HIP_H
 #define MARS5_HIP_H
 #include <stdint.h>
+#include "mars5_paged.h"
 
 /* The library is built with -fvisibility=hidden: only the entry points below are exported. */
 #define M5_API __attribute__((visibility("default")))
@@ -393,6 +394,16 @@ M5_API int m5_expand_tokens(const int64_t* tokens, int n, int n_text, const int3
 M5_API int m5_trim_bounds(const float* y, int n, int frame_length, int hop, float top_db, float* power, int n_frames,
                    int32_t* bounds, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Paged serving (mars5_paged.h: argument structures and semantics): block tables and slot maps from request lengths; q / k norms,
+ * rotation and the cache write; attention of new tokens over the paged cache; drafted tokens against the target's probabilities.
+ * ------------------------------------------------------------------------------------ */
+M5_API int m5_paged_plan(const M5PagedPlanArgs* a, void* stream);
+M5_API int m5_paged_rope_cache(int dtype, const M5PagedRopeArgs* a, void* stream);
+M5_API int m5_paged_attention(int dtype, const M5PagedAttnArgs* a, void* stream);
+M5_API int m5_paged_attention_workspace(int dtype, const M5PagedAttnArgs* a, int64_t* bytes);   /* host only, nothing is launched */
+M5_API int m5_draft_verify(int dtype, const M5DraftVerifyArgs* a, void* stream);
+
 M5_API int m5_add_int(int32_t* p, int32_t delta, void* stream);
 
 /* ------------------------------------------------------------------------------------
@@ -405,7 +416,7 @@ M5_API int m5_add_int(int32_t* p, int32_t delta, void* stream);
  * A plan is an array of ops in launch order; op.fn names an entry point of THIS header and op.a[] holds its arguments except
  * the trailing stream: integers by value, device pointers by address, floats as IEEE bits in the low 32, pointers to argument
  * structures (M5QkvScatter, M5DeferredLN, M5RowTiles, M5AttnArgs, M5GemvArgs, M5AttnDecodeArgs, M5ArMegaArgs, M5SampleArgs,
- * M5NarSampleArgs, M5NarUniformArgs) as (byte offset into `arena` + 1; 8-byte aligned), 0 = NULL.  Every argument of a step is a
+ * M5NarSampleArgs, M5NarUniformArgs, M5Paged*Args, M5DraftVerifyArgs) as (byte offset into `arena` + 1; 8-byte aligned), 0 = NULL.  Every argument of a step is a
  * pointer, stride or size (the step index, positions and RNG state live in device memory), so a session's plan is filled once
  * and serves every step; the caller owns ops / arena / all buffers and may capture the call in a hipGraph.  Returns the first
  * non-zero status of an op (the ops before it are already enqueued; *failed_op = its index, -1 on success, may be NULL);
@@ -416,7 +427,8 @@ enum {
     M5_FN_GEMM = 1, M5_FN_GEMM_EX, M5_FN_LAYERNORM, M5_FN_LAYERNORM_TWICE, M5_FN_LAYERNORM_MEAN, M5_FN_RMSNORM, M5_FN_ATTENTION,
     M5_FN_GATHER_ROWS, M5_FN_CHUNKED_EMBED, M5_FN_XATTN_ABSORB, M5_FN_XATTN_SCORES, M5_FN_XATTN_SCORES_EX, M5_FN_NAR_UNIFORMS,
     M5_FN_NAR_SAMPLE, M5_FN_ADD_INT, M5_FN_COPY_D2D, M5_FN_AR_GEMV, M5_FN_AR_ATTN_DECODE, M5_FN_AR_LAYERS_PERSISTENT, M5_FN_AR_SAMPLE,
-    M5_FN_AR_ROPE_CACHE_BATCH, M5_FN_AR_QKV_ROPE_BATCH, M5_FN_AR_ATTN_COMBINE_BATCH
+    M5_FN_AR_ROPE_CACHE_BATCH, M5_FN_AR_QKV_ROPE_BATCH, M5_FN_AR_ATTN_COMBINE_BATCH, M5_FN_PAGED_PLAN, M5_FN_PAGED_ROPE_CACHE,
+    M5_FN_PAGED_ATTENTION, M5_FN_DRAFT_VERIFY
 };
 typedef struct {
     int32_t fn, n_args;                 /* M5_FN_*, number of slots used (= the entry point's parameters without the stream) */

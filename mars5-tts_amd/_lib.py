@@ -145,6 +145,48 @@ class DeferredLN(C.Structure):
                 ("s", vp), ("s_bs", i64), ("eps", f32), ("n_feat", i32), ("rows_bs", i32)]
 
 
+class PagedPlanArgs(C.Structure):
+    """M5PagedPlanArgs (include/mars5_paged.h): block tables, slot map, positions and row offsets of one step."""
+    _fields_ = [("seq_len", vp), ("keep_len", vp), ("new_len", vp),
+                ("n_seq", i32), ("table_width", i32), ("n_blocks", i32), ("block_size", i32), ("n_rows", i32),
+                ("block_table", vp), ("table_rs", i64), ("free_blocks", vp), ("state", vp),
+                ("q_start", vp), ("slot_map", vp), ("positions", vp)]
+
+
+class PagedRopeArgs(C.Structure):
+    """M5PagedRopeArgs (include/mars5_paged.h): q / k norms, rotation and the paged cache write."""
+    _fields_ = [("qkv", vp), ("qkv_rs", i64), ("n_rows", i32), ("n_heads", i32), ("n_kv_heads", i32), ("head_dim", i32),
+                ("q_norm", vp), ("k_norm", vp), ("eps", f32),
+                ("rope", vp), ("n_pos", i32), ("n_pairs", i32), ("interleaved", i32),
+                ("positions", vp), ("slot_map", vp),
+                ("q_out", vp), ("q_rs", i64), ("q_hs", i64),
+                ("k_cache", vp), ("k_bs", i64), ("k_hs", i64), ("k_ss", i64),
+                ("v_cache", vp), ("v_bs", i64), ("v_hs", i64), ("v_ss", i64),
+                ("n_blocks", i32), ("block_size", i32)]
+
+
+class PagedAttnArgs(C.Structure):
+    """M5PagedAttnArgs (include/mars5_paged.h): attention of new tokens over a paged cache."""
+    _fields_ = [("q", vp), ("q_rs", i64), ("q_hs", i64),
+                ("k_cache", vp), ("k_bs", i64), ("k_hs", i64), ("k_ss", i64),
+                ("v_cache", vp), ("v_bs", i64), ("v_hs", i64), ("v_ss", i64),
+                ("block_table", vp), ("table_rs", i64), ("table_width", i32), ("n_blocks", i32), ("block_size", i32),
+                ("n_seq", i32), ("n_rows", i32), ("max_new", i32), ("n_heads", i32), ("n_kv_heads", i32), ("head_dim", i32), ("window", i32),
+                ("seq_len", vp), ("q_start", vp), ("scale", f32),
+                ("out", vp), ("o_rs", i64), ("o_hs", i64), ("workspace", vp), ("workspace_bytes", i64)]
+
+
+class DraftVerifyArgs(C.Structure):
+    """M5DraftVerifyArgs (include/mars5_paged.h): drafted tokens against the target's probabilities."""
+    _fields_ = [("target", vp), ("t_rs", i64), ("draft", vp), ("d_rs", i64),
+                ("n_rows", i32), ("vocab", i32), ("n_seq", i32), ("out_width", i32),
+                ("tokens", vp), ("row_start", vp), ("uniforms", vp), ("noise", vp), ("noise_rs", i64),
+                ("out_tokens", vp), ("out_rs", i64), ("n_out", vp), ("seq_len", vp), ("keep_len", vp),
+                ("workspace", vp), ("workspace_bytes", i64)]
+
+
+PST_FREE, PST_STATUS, PST_ROWS, PST_WORDS = 0, 1, 2, 8
+DRAFT_WS_BYTES = 32
 PLAN_MAX_ARGS = 24
 
 
@@ -163,7 +205,7 @@ PLAN_FN = {name: i + 1 for i, name in enumerate([
     "m5_gemm", "m5_gemm_ex", "m5_layernorm", "m5_layernorm_twice", "m5_layernorm_mean", "m5_rmsnorm", "m5_attention", "m5_gather_rows",
     "m5_chunked_embed", "m5_xattn_absorb", "m5_xattn_scores", "m5_xattn_scores_ex", "m5_nar_uniforms", "m5_nar_sample", "m5_add_int",
     "m5_copy_d2d", "m5_ar_gemv", "m5_ar_attn_decode", "m5_ar_layers_persistent", "m5_ar_sample", "m5_ar_rope_cache_batch",
-    "m5_ar_qkv_rope_batch", "m5_ar_attn_combine_batch"])}
+    "m5_ar_qkv_rope_batch", "m5_ar_attn_combine_batch", "m5_paged_plan", "m5_paged_rope_cache", "m5_paged_attention", "m5_draft_verify"])}
 
 # name -> (restype, argtypes); also the list the symbol-export test checks against the header
 PROTOTYPES = {
@@ -197,6 +239,11 @@ PROTOTYPES = {
     "m5_nar_uniforms": (C.c_int, [C.POINTER(NarUniformArgs), vp]),
     "m5_expand_tokens": (C.c_int, [vp, C.c_int, C.c_int, vp, vp, C.c_int, vp, C.c_int, vp, vp]),
     "m5_trim_bounds": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, f32, vp, C.c_int, vp, vp]),
+    "m5_paged_plan": (C.c_int, [C.POINTER(PagedPlanArgs), vp]),
+    "m5_paged_rope_cache": (C.c_int, [C.c_int, C.POINTER(PagedRopeArgs), vp]),
+    "m5_paged_attention": (C.c_int, [C.c_int, C.POINTER(PagedAttnArgs), vp]),
+    "m5_paged_attention_workspace": (C.c_int, [C.c_int, C.POINTER(PagedAttnArgs), C.POINTER(i64)]),
+    "m5_draft_verify": (C.c_int, [C.c_int, C.POINTER(DraftVerifyArgs), vp]),
     "m5_add_int": (C.c_int, [vp, i32, vp]),
     "m5_copy_d2d": (C.c_int, [vp, vp, i64, vp]),
     "m5_nar_step": (C.c_int, [C.POINTER(StagePlanC), vp]),

@@ -7,13 +7,13 @@
 set -e
 cd "$(dirname "$0")"
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -ffp-contract=off -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
-SRCS="gemm gemm16 gemm_skinny attention attention16 xattn_absorb rowops ar_decode ar_mega ar_batch nar_sample util stage_plan"
+SRCS="gemm gemm16 gemm_skinny attention attention16 xattn_absorb rowops ar_decode ar_mega ar_batch nar_sample util stage_plan paged paged_attention draft_verify"
 build_one() {   # $1 = object dir, $2 = extra flags, $3 = output library
   mkdir -p $1
   pids=()
   for f in $SRCS; do
     stale=0
-    for h in *.h ../../include/mars5_hip.h; do [ $h -nt $1/$f.o ] && stale=1; done
+    for h in *.h ../../include/*.h; do [ $h -nt $1/$f.o ] && stale=1; done
     if [ ! -f $1/$f.o ] || [ $f.hip -nt $1/$f.o ] || [ $stale = 1 ]; then
       hipcc $FLAGS $2 -c $f.hip -o $1/$f.o &
       pids+=($!)

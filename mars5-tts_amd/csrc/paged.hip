@@ -1,0 +1,269 @@
+// Paged KV cache: the step's block tables / slot map / positions (m5_paged_plan) and the pass that norms and rotates the new q and
+// k heads and writes k and v into the cache (m5_paged_rope_cache).  Semantics: include/mars5_paged.h.
+#include "common.h"
+#include "paged_index.h"
+#include <limits.h>
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------- m5_paged_plan
+// Every workgroup scans the requests itself (three prefix sums into LDS: rows, blocks taken, blocks given back), so the rows and
+// blocks can be dealt to many workgroups without a second launch.  Nothing that any workgroup reads is written before the end:
+// table entries written lie behind the pages a growing request holds, those read as "given back" behind the pages a shrinking one
+// keeps, free-list entries written lie at or above n_free and those read below.  seq_len and the state words are written by the
+// workgroup that finishes last (ticket word of the state; it leaves the ticket at 0).
+constexpr int PLAN_NT = 1024;
+constexpr int PLAN_MAX_SEQ = 8192;
+
+__device__ inline int64_t wave_scan(int64_t v) {             // inclusive
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t o = __shfl_up((long long)v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+__global__ __launch_bounds__(PLAN_NT) void paged_plan_kernel(M5PagedPlanArgs p, int shift) {
+    extern __shared__ int pre[];                             // [3][n_seq + 1]
+    __shared__ int64_t wsum[3][PLAN_NT / 64];
+    __shared__ int first_bad, last;
+    const int B = p.n_seq, tid = threadIdx.x, wave = tid >> 6;
+    int* row_pre = pre;
+    int* take_pre = pre + (B + 1);
+    int* give_pre = pre + 2 * (B + 1);
+    if (tid == 0) first_bad = INT_MAX;
+    const int n_free = m5_clampi(p.state[M5_PST_FREE], 0, p.n_blocks);
+    __syncthreads();
+
+    const int per = (B + PLAN_NT - 1) / PLAN_NT;             // consecutive requests per thread
+    const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
+    int64_t rows = 0, take = 0, give = 0;
+    for (int b = b0; b < b1; ++b) {
+        int have, need;
+        const int add = p.new_len[b];
+        if (!m5_plan_request(p.seq_len[b], p.keep_len[b], add, p.table_width, shift, have, need)) { atomicMin(&first_bad, b); continue; }
+        rows += add;
+        take += max(need - have, 0);
+        give += max(have - need, 0);
+    }
+    const int64_t ri = wave_scan(rows), ti = wave_scan(take), gi = wave_scan(give);
+    if ((tid & 63) == 63) { wsum[0][wave] = ri; wsum[1][wave] = ti; wsum[2][wave] = gi; }
+    __syncthreads();
+    int64_t rb = 0, tb = 0, gb = 0, n_rows = 0, n_take = 0, n_give = 0;
+    for (int w = 0; w < PLAN_NT / 64; ++w) {
+        if (w == wave) { rb = n_rows; tb = n_take; gb = n_give; }
+        n_rows += wsum[0][w];
+        n_take += wsum[1][w];
+        n_give += wsum[2][w];
+    }
+    int status = 0;
+    if (first_bad != INT_MAX) status = -1 - first_bad;
+    else if (n_rows > (p.slot_map ? p.n_rows : INT_MAX)) status = -1 - B;
+    else if (n_free + n_give - n_take > p.n_blocks) status = -2 - B;
+    else if (n_take > n_free + n_give) status = (int)(n_take - n_free - n_give);
+    const bool ok = status == 0;                             // uniform over the grid
+    rb = ok ? rb + ri - rows : 0;
+    tb = ok ? tb + ti - take : 0;
+    gb = ok ? gb + gi - give : 0;
+    for (int b = b0; b < b1; ++b) {                          // exclusive prefixes
+        row_pre[b] = (int)rb; take_pre[b] = (int)tb; give_pre[b] = (int)gb;
+        int have, need;
+        const int add = p.new_len[b];
+        m5_plan_request(p.seq_len[b], p.keep_len[b], add, p.table_width, shift, have, need);
+        if (ok) { rb += add; tb += max(need - have, 0); gb += max(have - need, 0); }
+    }
+    if (tid == PLAN_NT - 1) { row_pre[B] = ok ? (int)n_rows : 0; take_pre[B] = ok ? (int)n_take : 0; give_pre[B] = ok ? (int)n_give : 0; }
+    __syncthreads();
+
+    const int taken = ok ? (int)n_take : 0, given = ok ? (int)n_give : 0, described = ok ? (int)n_rows : 0;
+    auto returned = [&](int i) {                             // id of returned page i
+        const int b = m5_upper(give_pre, B, i);
+        const int need = m5_pages(p.keep_len[b] + p.new_len[b], shift);
+        return p.block_table[(int64_t)b * p.table_rs + need + (i - give_pre[b])];
+    };
+    auto allocation = [&](int a) {                           // id of allocation a
+        const int src = m5_plan_source(a, given, n_free);
+        return src >= 0 ? p.free_blocks[src] : returned(-1 - src);
+    };
+    const int gt = blockIdx.x * PLAN_NT + tid, gn = gridDim.x * PLAN_NT;
+    if (p.slot_map) {
+        for (int r = gt; r < p.n_rows; r += gn) {
+            int slot = -1, pos = -1;
+            if (r < described) {
+                const int b = m5_upper(row_pre, B, r);
+                pos = p.keep_len[b] + (r - row_pre[b]);
+                const int page = pos >> shift, have = m5_pages(p.seq_len[b], shift);
+                const int id = page < have ? p.block_table[(int64_t)b * p.table_rs + page] : allocation(take_pre[b] + (page - have));
+                if (m5_block(id, p.n_blocks) >= 0) slot = (id << shift) + (pos & ((1 << shift) - 1));
+            }
+            p.slot_map[r] = slot;
+            p.positions[r] = pos;
+        }
+    }
+    for (int a = gt; a < taken; a += gn) {
+        const int b = m5_upper(take_pre, B, a);
+        p.block_table[(int64_t)b * p.table_rs + m5_pages(p.seq_len[b], shift) + (a - take_pre[b])] = allocation(a);
+    }
+    for (int i = taken + gt; i < given; i += gn) p.free_blocks[m5_plan_push(i, given, n_free)] = returned(i);
+    if (blockIdx.x == 0)
+        for (int b = tid; b <= B; b += PLAN_NT) p.q_start[b] = row_pre[b];
+
+    __syncthreads();                                         // this workgroup has read all that it will of seq_len and the state
+    if (tid == 0)
+        last = gridDim.x == 1 ||
+               __hip_atomic_fetch_add(&p.state[M5_PST_ROWS + 1], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    if (ok)
+        for (int b = tid; b < B; b += PLAN_NT) p.seq_len[b] = p.keep_len[b] + p.new_len[b];
+    if (tid == 0) {
+        p.state[M5_PST_FREE] = n_free + given - taken;
+        p.state[M5_PST_STATUS] = status;
+        p.state[M5_PST_ROWS] = described;
+        p.state[M5_PST_ROWS + 1] = 0;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- m5_paged_rope_cache
+// A group of head_dim / EPL lanes holds one head, 16 bytes per lane: the sum of squares is a few cross-lane adds, an adjacent pair
+// lies in one lane, a half-split pair in two lanes n_pairs / EPL apart.  A group keeps its row's cosines and sines in registers
+// and walks heads of that row.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void paged_rope_kernel(M5PagedRopeArgs p, int shift) {
+    using st = typename T::storage;
+    constexpr int E = T::EPL, L = HD / E, G = 256 / L;       // elements per lane, lanes per head, heads per workgroup at a time
+    const int row = blockIdx.x, tid = threadIdx.x, l = tid % L, g = tid / L;
+    const int pos = p.positions[row], slot = p.slot_map[row];
+    if (pos < 0 || pos >= p.n_pos || slot < 0 || (slot >> shift) >= p.n_blocks) return;        // padding (workgroup-uniform)
+    const int e0 = l * E, heads = p.n_heads + 2 * p.n_kv_heads;
+    const bool turns = e0 < 2 * p.n_pairs;                   // n_pairs is a multiple of 8: a lane's elements all turn or none do
+    const float* cs = p.rope + (int64_t)pos * p.n_pairs * 2;
+    float c[E], s[E];
+    const bool second = !p.interleaved && e0 >= p.n_pairs;
+#pragma unroll
+    for (int i = 0; i < E; ++i) { c[i] = 1.f; s[i] = 0.f; }
+    if (turns) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int pair = p.interleaved ? (e0 + i) >> 1 : (second ? e0 + i - p.n_pairs : e0 + i);
+            c[i] = cs[2 * pair];
+            s[i] = cs[2 * pair + 1];
+        }
+    }
+    const int partner = ((tid & 63) & ~(L - 1)) + (second ? l - p.n_pairs / E : l + p.n_pairs / E) % L;
+    const int64_t blk = slot >> shift, off = slot & ((1 << shift) - 1);
+    const int h0 = blockIdx.y * G, hn = min(h0 + (int)G, heads);
+    for (int hb = h0; hb < hn; hb += G) {
+        const int h = hb + g;
+        const bool live = h < heads;
+        Vec16<T> v;
+        v.zero();
+        if (live) v.load((const st*)p.qkv + (int64_t)row * p.qkv_rs + (int64_t)h * HD + e0);
+        const bool is_v = h >= p.n_heads + p.n_kv_heads, is_q = h < p.n_heads;
+        float x[E];
+        v.to_float(x);
+        const float* w = is_q ? p.q_norm : p.k_norm;
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) ss = fmaf(x[i], x[i], ss);
+        ss += lane_xor1(ss);
+        ss += lane_xor2(ss);
+        ss += lane_xor4(ss);
+        if (L >= 16) ss += lane_xor8(ss);
+        if (L >= 32) ss += lane_xor16(ss);
+        if (w && !is_v) {
+            const float r = 1.0f / sqrtf(ss * (1.0f / HD) + p.eps);
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = x[i] * r * w[e0 + i];
+        }
+        float y[E];
+        if (p.interleaved) {
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                y[i] = x[i] * c[i] - x[i + 1] * s[i];
+                y[i + 1] = x[i] * s[i] + x[i + 1] * c[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float o = __shfl(x[i], partner);
+                y[i] = second ? o * s[i] + x[i] * c[i] : x[i] * c[i] - o * s[i];
+            }
+        }
+        if (!is_v && turns) {
+            uint4 raw;
+            st* out = reinterpret_cast<st*>(&raw);
+#pragma unroll
+            for (int i = 0; i < E; ++i) out[i] = T::from_f32(y[i]);
+            v.raw = raw;
+        } else if (!is_v) {
+            uint4 raw;
+            st* out = reinterpret_cast<st*>(&raw);
+#pragma unroll
+            for (int i = 0; i < E; ++i) out[i] = T::from_f32(x[i]);
+            v.raw = raw;
+        }
+        if (!live) continue;
+        st* dst;
+        if (is_q) dst = (st*)p.q_out + (int64_t)row * p.q_rs + (int64_t)h * p.q_hs;
+        else if (!is_v) dst = (st*)p.k_cache + blk * p.k_bs + (int64_t)(h - p.n_heads) * p.k_hs + off * p.k_ss;
+        else dst = (st*)p.v_cache + blk * p.v_bs + (int64_t)(h - p.n_heads - p.n_kv_heads) * p.v_hs + off * p.v_ss;
+        *reinterpret_cast<uint4*>(dst + e0) = v.raw;
+    }
+}
+
+template <typename T>
+int launch_rope(const M5PagedRopeArgs& a, int shift, hipStream_t s) {
+    const int per = 256 / (a.head_dim / T::EPL), heads = a.n_heads + 2 * a.n_kv_heads;
+    const dim3 grid(a.n_rows, (heads + per - 1) / per);
+    if (a.head_dim == 64) hipLaunchKernelGGL((paged_rope_kernel<T, 64>), grid, dim3(256), 0, s, a, shift);
+    else hipLaunchKernelGGL((paged_rope_kernel<T, 128>), grid, dim3(256), 0, s, a, shift);
+    M5_CHECK_LAUNCH();
+    return M5_OK;
+}
+
+bool aligned(const void* p, int64_t a, int64_t b, int64_t c, int epl) {
+    return ((uintptr_t)p & 15) == 0 && a % epl == 0 && b % epl == 0 && c % epl == 0;
+}
+
+}  // namespace
+
+extern "C" int m5_paged_plan(const M5PagedPlanArgs* a, void* stream) {
+    if (!a || !a->seq_len || !a->keep_len || !a->new_len || !a->block_table || !a->free_blocks || !a->state || !a->q_start) return M5_ERR_ARG;
+    const int shift = m5_log2(a->block_size);
+    if (a->n_seq <= 0 || a->table_width <= 0 || a->n_blocks <= 0 || shift < 0 || a->table_rs < a->table_width) return M5_ERR_ARG;
+    if (!a->slot_map != !a->positions || (a->slot_map && a->n_rows < 0)) return M5_ERR_ARG;
+    // positions, slots and (request, page) pairs are counted in 32 bits
+    if (a->n_seq > PLAN_MAX_SEQ || a->block_size > 1024 || ((int64_t)a->table_width << shift) > INT_MAX || ((int64_t)a->n_blocks << shift) > INT_MAX ||
+        (int64_t)a->n_seq * a->table_width > INT_MAX)
+        return M5_ERR_UNSUPPORTED;
+    const int lds = 3 * (a->n_seq + 1) * (int)sizeof(int);
+    if (lds > 48 * 1024 &&
+        hipFuncSetAttribute((const void*)paged_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 3 * (PLAN_MAX_SEQ + 1) * (int)sizeof(int)) != hipSuccess)
+        return M5_ERR_LAUNCH;
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(PLAN_NT), lds, (hipStream_t)stream, *a, shift);
+    M5_CHECK_LAUNCH();
+    return M5_OK;
+}
+
+extern "C" int m5_paged_rope_cache(int dtype, const M5PagedRopeArgs* a, void* stream) {
+    if (!a || !a->qkv || !a->rope || !a->positions || !a->slot_map || !a->q_out || !a->k_cache || !a->v_cache) return M5_ERR_ARG;
+    const int shift = m5_log2(a->block_size);
+    if (a->n_rows < 0 || a->n_heads <= 0 || a->n_kv_heads <= 0 || a->n_pos <= 0 || a->n_blocks <= 0 || shift < 0) return M5_ERR_ARG;
+    if (dtype != M5_F32 && dtype != M5_F16 && dtype != M5_BF16) return M5_ERR_UNSUPPORTED;
+    if ((a->head_dim != 64 && a->head_dim != 128) || a->block_size > 1024 || ((int64_t)a->n_blocks << shift) > INT_MAX) return M5_ERR_UNSUPPORTED;
+    if (a->n_pairs <= 0 || a->n_pairs % 8 || 2 * a->n_pairs > a->head_dim) return M5_ERR_UNSUPPORTED;
+    const int epl = dtype == M5_F32 ? 4 : 8;
+    if (!aligned(a->qkv, a->qkv_rs, 0, 0, epl) || !aligned(a->q_out, a->q_rs, a->q_hs, 0, epl) || !aligned(a->k_cache, a->k_bs, a->k_hs, a->k_ss, epl) ||
+        !aligned(a->v_cache, a->v_bs, a->v_hs, a->v_ss, epl) || ((uintptr_t)a->rope & 15) || ((uintptr_t)a->q_norm & 15) || ((uintptr_t)a->k_norm & 15))
+        return M5_ERR_UNSUPPORTED;
+    if (a->n_rows == 0) return M5_OK;
+    hipStream_t s = (hipStream_t)stream;
+    switch (dtype) {
+        case M5_F32: return launch_rope<F32T>(*a, shift, s);
+        case M5_F16: return launch_rope<F16T>(*a, shift, s);
+        default: return launch_rope<BF16T>(*a, shift, s);
+    }
+}

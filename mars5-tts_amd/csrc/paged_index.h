@@ -1,0 +1,66 @@
+// Index arithmetic of the paged KV cache (paged.hip, paged_attention.hip, draft_verify.hip).  Everything that a kernel derives
+// from DEVICE data (lengths, block ids, row offsets: no host check can see them) is clamped or refused here, so that no value of
+// theirs leads outside a buffer.  Plain C++: tests/test_paged_cpu.py compiles this text with g++.
+#pragma once
+#include <stdint.h>
+#ifdef __HIPCC__
+#define M5_HD __host__ __device__ static inline
+#else
+#define M5_HD static inline
+#endif
+
+M5_HD int m5_clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+
+// log2 of a power of two, -1 for any other value
+M5_HD int m5_log2(int v) {
+    if (v <= 0 || (v & (v - 1))) return -1;
+    int s = 0;
+    while ((1 << s) < v) ++s;
+    return s;
+}
+
+// pages that hold n positions
+M5_HD int m5_pages(int n, int shift) { return (int)(((int64_t)n + (1 << shift) - 1) >> shift); }
+
+// a block id as the kernels use it: the id, or -1 for one outside the cache
+M5_HD int m5_block(int id, int n_blocks) { return (id >= 0 && id < n_blocks) ? id : -1; }
+
+// One request of a launch: its rows [r0, r1) of the packed buffers and the positions that the cache holds for it, cut down to what
+// the buffers hold (n_rows rows, cap = table_width * block_size positions).  Query row r stands at position len - (r1 - r).
+struct M5Request { int r0, r1, len; };
+M5_HD M5Request m5_request(int start, int end, int seq_len, int n_rows, int64_t cap) {
+    M5Request q;
+    q.r0 = m5_clampi(start, 0, n_rows);
+    q.r1 = m5_clampi(end, q.r0, n_rows);
+    q.len = seq_len < 0 ? 0 : (seq_len > cap ? (int)cap : seq_len);
+    return q;
+}
+
+// Keys that the query at position `pos` of a request with `len` cached positions sees: [lo, hi), empty when lo >= hi.
+M5_HD int m5_key_hi(int pos, int len) { return pos + 1 < len ? pos + 1 : len; }
+M5_HD int m5_key_lo(int pos, int window) { return (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0; }
+
+// paged_plan, one request: pages held before, pages needed after; false when the request is not a valid one.
+M5_HD bool m5_plan_request(int held, int keep, int add, int width, int shift, int& have, int& need) {
+    const int64_t end = (int64_t)keep + add;
+    const bool ok = held >= 0 && keep >= 0 && add >= 0 && keep <= held && end <= ((int64_t)width << shift) && held <= ((int64_t)width << shift);
+    have = ok ? m5_pages(held, shift) : 0;
+    need = ok ? m5_pages((int)end, shift) : 0;
+    return ok;
+}
+// Free stack of n_free ids, R pages returned this call (numbered upwards by request, then page), allocation number a.  Pages are
+// pushed from the last to the first and popped from the top, so allocation a takes returned page a while there is one, then the
+// old stack from its top.  >= 0: index into the free list; < 0: returned page -1 - result.
+M5_HD int m5_plan_source(int a, int returned, int n_free) { return a < returned ? -1 - a : n_free - 1 - (a - returned); }
+// position in the free list of returned page i (only those with i >= pages taken stay there)
+M5_HD int m5_plan_push(int i, int returned, int n_free) { return n_free + returned - 1 - i; }
+
+// Index of the last entry of the non-decreasing pre[0 .. n] (pre[0] = 0 <= v < pre[n]) that is <= v.
+M5_HD int m5_upper(const int* pre, int n, int v) {
+    int lo = 0, hi = n;                       // pre[lo] <= v < pre[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= v) lo = mid; else hi = mid;
+    }
+    return lo;
+}

@@ -98,6 +98,10 @@ int run_op(const M5PlanOp& op, const M5StagePlan* plan, void* stream, unsigned a
         M5_OP(M5_FN_AR_ROPE_CACHE_BATCH, m5_ar_rope_cache_batch, KIND_AR)
         M5_OP(M5_FN_AR_QKV_ROPE_BATCH, m5_ar_qkv_rope_batch, KIND_AR)
         M5_OP(M5_FN_AR_ATTN_COMBINE_BATCH, m5_ar_attn_combine_batch, KIND_AR)
+        M5_OP(M5_FN_PAGED_PLAN, m5_paged_plan, KIND_AR)
+        M5_OP(M5_FN_PAGED_ROPE_CACHE, m5_paged_rope_cache, KIND_AR)
+        M5_OP(M5_FN_PAGED_ATTENTION, m5_paged_attention, KIND_AR)
+        M5_OP(M5_FN_DRAFT_VERIFY, m5_draft_verify, KIND_AR)
         default: return M5_ERR_ARG;
     }
 #undef M5_OP
