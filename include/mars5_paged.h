@@ -67,7 +67,7 @@ typedef struct {
  * workspace (may be NULL): scratch for keys split over workgroups when there are few rows; zero-filled once by the caller,
  * left ready for the next call; calls that may run at the same time need one each; 16-byte aligned.  More bytes allow more
  * splits; m5_paged_attention_workspace tells how many bytes the largest split of these shapes uses.
- * head_dim 64 or 128; n_seq <= 8192; pointers and strides multiples of 16 bytes. */
+ * head_dim 64 or 128; n_seq <= 4096; at most 2^30 positions per table row; pointers and strides multiples of 16 bytes. */
 typedef struct {
     const void* q; int64_t q_rs, q_hs;
     const void* k_cache; int64_t k_bs, k_hs, k_ss;
