@@ -128,98 +128,120 @@ __global__ __launch_bounds__(PLAN_NT) void paged_plan_kernel(M5PagedPlanArgs p, 
 
 // ---------------------------------------------------------------------------------------------------- m5_paged_rope_cache
 // A group of head_dim / EPL lanes holds one head, 16 bytes per lane: the sum of squares is a few cross-lane adds, an adjacent pair
-// lies in one lane, a half-split pair in two lanes n_pairs / EPL apart.  A group keeps its row's cosines and sines in registers
-// and walks heads of that row.
-template <typename T, int HD>
+// lies in one lane, a half-split pair in two lanes n_pairs / EPL apart.  A workgroup walks the heads of one row, U per group with their
+// loads in flight together; the row's cosines and sines and the norm weights stay in registers.
+template <typename T, int HD, bool INTER, int U>
 __global__ __launch_bounds__(256) void paged_rope_kernel(M5PagedRopeArgs p, int shift) {
     using st = typename T::storage;
-    constexpr int E = T::EPL, L = HD / E, G = 256 / L;       // elements per lane, lanes per head, heads per workgroup at a time
+    constexpr int E = T::EPL, L = HD / E, G = 256 / L;       // elements per lane, lanes per head, heads at a time
     const int row = blockIdx.x, tid = threadIdx.x, l = tid % L, g = tid / L;
+    const int e0 = l * E, n_qk = p.n_heads + p.n_kv_heads, heads = n_qk + p.n_kv_heads;
+    const int first = blockIdx.y * (U * G);
+    const st* src = (const st*)p.qkv + (int64_t)row * p.qkv_rs + e0;
+    Vec16<T> v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {                            // requested before anything is waited for
+        v[k].zero();
+        if (first + k * G + g < heads) v[k].load(src + (int64_t)(first + k * G + g) * HD);
+    }
     const int pos = p.positions[row], slot = p.slot_map[row];
     if (pos < 0 || pos >= p.n_pos || slot < 0 || (slot >> shift) >= p.n_blocks) return;        // padding (workgroup-uniform)
-    const int e0 = l * E, heads = p.n_heads + 2 * p.n_kv_heads;
     const bool turns = e0 < 2 * p.n_pairs;                   // n_pairs is a multiple of 8: a lane's elements all turn or none do
-    const float* cs = p.rope + (int64_t)pos * p.n_pairs * 2;
-    float c[E], s[E];
-    const bool second = !p.interleaved && e0 >= p.n_pairs;
+    const bool second = !INTER && e0 >= p.n_pairs;
+    constexpr int NC = INTER ? E / 2 : E;                    // pairs of a lane
+    float c[NC], s[NC];
+    {
+        const int pair = INTER ? e0 >> 1 : (second ? e0 - p.n_pairs : e0);
+        const float4* cs = reinterpret_cast<const float4*>(p.rope + ((int64_t)pos * p.n_pairs + (turns ? pair : 0)) * 2);
 #pragma unroll
-    for (int i = 0; i < E; ++i) { c[i] = 1.f; s[i] = 0.f; }
-    if (turns) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int pair = p.interleaved ? (e0 + i) >> 1 : (second ? e0 + i - p.n_pairs : e0 + i);
-            c[i] = cs[2 * pair];
-            s[i] = cs[2 * pair + 1];
+        for (int i = 0; i < NC; i += 2) {
+            const float4 t = turns ? cs[i / 2] : make_float4(1.f, 0.f, 1.f, 0.f);
+            c[i] = t.x;
+            s[i] = second ? -t.y : t.y;
+            c[i + 1] = t.z;
+            s[i + 1] = second ? -t.w : t.w;
         }
     }
-    const int partner = ((tid & 63) & ~(L - 1)) + (second ? l - p.n_pairs / E : l + p.n_pairs / E) % L;
+    const int apart = p.n_pairs / E;
+    const int partner = ((tid & 63) & ~(L - 1)) + (second ? l - apart : l + apart) % L;
     const int64_t blk = slot >> shift, off = slot & ((1 << shift) - 1);
-    const int h0 = blockIdx.y * G, hn = min(h0 + (int)G, heads);
-    for (int hb = h0; hb < hn; hb += G) {
-        const int h = hb + g;
-        const bool live = h < heads;
-        Vec16<T> v;
-        v.zero();
-        if (live) v.load((const st*)p.qkv + (int64_t)row * p.qkv_rs + (int64_t)h * HD + e0);
-        const bool is_v = h >= p.n_heads + p.n_kv_heads, is_q = h < p.n_heads;
-        float x[E];
-        v.to_float(x);
-        const float* w = is_q ? p.q_norm : p.k_norm;
-        float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) ss = fmaf(x[i], x[i], ss);
-        ss += lane_xor1(ss);
-        ss += lane_xor2(ss);
-        ss += lane_xor4(ss);
-        if (L >= 16) ss += lane_xor8(ss);
-        if (L >= 32) ss += lane_xor16(ss);
-        if (w && !is_v) {
-            const float r = 1.0f / sqrtf(ss * (1.0f / HD) + p.eps);
+    for (int k = 0; k < U; ++k) {
+        const int h = first + k * G + g;
+        if (h - g >= heads) break;                           // (uniform)
+        const bool is_q = h < p.n_heads, is_v = h >= n_qk;
+        if (h - g < n_qk) {                                  // some group here holds a q or k head
+            float x[E], y[E];
+            v[k].to_float(x);
+            const float* w = is_q ? p.q_norm : p.k_norm;
+            if (p.q_norm || p.k_norm) {
+                float ss = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = x[i] * r * w[e0 + i];
-        }
-        float y[E];
-        if (p.interleaved) {
+                for (int i = 0; i < E; ++i) ss = fmaf(x[i], x[i], ss);
+                ss += lane_xor1(ss);
+                ss += lane_xor2(ss);
+                ss += lane_xor4(ss);
+                if (L >= 16) ss += lane_xor8(ss);
+                if (L >= 32) ss += lane_xor16(ss);
+                if (w) {
+                    const float r = 1.0f / sqrtf(ss * (1.0f / HD) + p.eps);
 #pragma unroll
-            for (int i = 0; i < E; i += 2) {
-                y[i] = x[i] * c[i] - x[i + 1] * s[i];
-                y[i + 1] = x[i] * s[i] + x[i + 1] * c[i];
+                    for (int i = 0; i < E; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(w + e0 + i);
+                        x[i] = x[i] * r * f.x;
+                        x[i + 1] = x[i + 1] * r * f.y;
+                        x[i + 2] = x[i + 2] * r * f.z;
+                        x[i + 3] = x[i + 3] * r * f.w;
+                    }
+                }
             }
-        } else {
+            if constexpr (INTER) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float o = __shfl(x[i], partner);
-                y[i] = second ? o * s[i] + x[i] * c[i] : x[i] * c[i] - o * s[i];
+                for (int i = 0; i < E; i += 2) {
+                    y[i] = x[i] * c[i / 2] - x[i + 1] * s[i / 2];
+                    y[i + 1] = x[i] * s[i / 2] + x[i + 1] * c[i / 2];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) {                // (second half: s holds -sin, so both halves are x cos - partner s)
+                    const float o = apart == 8 ? lane_xor8(x[i]) : (apart == 4 ? lane_xor4(x[i]) : __shfl(x[i], partner));
+                    y[i] = x[i] * c[i] - o * s[i];
+                }
+            }
+            if (!is_v) {
+                st out[E];
+#pragma unroll
+                for (int i = 0; i < E; ++i) out[i] = T::from_f32(turns ? y[i] : x[i]);
+                v[k].raw = *reinterpret_cast<const uint4*>(out);
             }
         }
-        if (!is_v && turns) {
-            uint4 raw;
-            st* out = reinterpret_cast<st*>(&raw);
-#pragma unroll
-            for (int i = 0; i < E; ++i) out[i] = T::from_f32(y[i]);
-            v.raw = raw;
-        } else if (!is_v) {
-            uint4 raw;
-            st* out = reinterpret_cast<st*>(&raw);
-#pragma unroll
-            for (int i = 0; i < E; ++i) out[i] = T::from_f32(x[i]);
-            v.raw = raw;
-        }
-        if (!live) continue;
+        if (h >= heads) continue;
         st* dst;
         if (is_q) dst = (st*)p.q_out + (int64_t)row * p.q_rs + (int64_t)h * p.q_hs;
         else if (!is_v) dst = (st*)p.k_cache + blk * p.k_bs + (int64_t)(h - p.n_heads) * p.k_hs + off * p.k_ss;
-        else dst = (st*)p.v_cache + blk * p.v_bs + (int64_t)(h - p.n_heads - p.n_kv_heads) * p.v_hs + off * p.v_ss;
-        *reinterpret_cast<uint4*>(dst + e0) = v.raw;
+        else dst = (st*)p.v_cache + blk * p.v_bs + (int64_t)(h - n_qk) * p.v_hs + off * p.v_ss;
+        *reinterpret_cast<uint4*>(dst + e0) = v[k].raw;
     }
 }
 
+template <typename T, int HD, int U>
+void launch_rope_u(const M5PagedRopeArgs& a, int shift, hipStream_t s) {
+    const int per = 256 / (HD / T::EPL) * U;                 // heads of a workgroup
+    const dim3 grid(a.n_rows, (a.n_heads + 2 * a.n_kv_heads + per - 1) / per);
+    if (a.interleaved) hipLaunchKernelGGL((paged_rope_kernel<T, HD, true, U>), grid, dim3(256), 0, s, a, shift);
+    else hipLaunchKernelGGL((paged_rope_kernel<T, HD, false, U>), grid, dim3(256), 0, s, a, shift);
+}
+template <typename T, int HD>
+void launch_rope_hd(const M5PagedRopeArgs& a, int shift, hipStream_t s) {
+    // Few rows: more, shorter workgroups (37 rows of 72 heads of 64: 2.9 us against 3.7).  Many: a row's table values serve four heads
+    // (16384 rows of 48 heads of 128: 83 us, 4.9 TB/s, against 109); equal at about 1000 rows (5.7 / 5.9 us, 9.2 / 8.7 us).
+    if (a.n_rows < 1024) launch_rope_u<T, HD, 1>(a, shift, s);
+    else launch_rope_u<T, HD, 4>(a, shift, s);
+}
 template <typename T>
 int launch_rope(const M5PagedRopeArgs& a, int shift, hipStream_t s) {
-    const int per = 256 / (a.head_dim / T::EPL), heads = a.n_heads + 2 * a.n_kv_heads;
-    const dim3 grid(a.n_rows, (heads + per - 1) / per);
-    if (a.head_dim == 64) hipLaunchKernelGGL((paged_rope_kernel<T, 64>), grid, dim3(256), 0, s, a, shift);
-    else hipLaunchKernelGGL((paged_rope_kernel<T, 128>), grid, dim3(256), 0, s, a, shift);
+    if (a.head_dim == 64) launch_rope_hd<T, 64>(a, shift, s);
+    else launch_rope_hd<T, 128>(a, shift, s);
     M5_CHECK_LAUNCH();
     return M5_OK;
 }
@@ -243,7 +265,10 @@ extern "C" int m5_paged_plan(const M5PagedPlanArgs* a, void* stream) {
     if (lds > 48 * 1024 &&
         hipFuncSetAttribute((const void*)paged_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 3 * (PLAN_MAX_SEQ + 1) * (int)sizeof(int)) != hipSuccess)
         return M5_ERR_LAUNCH;
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(PLAN_NT), lds, (hipStream_t)stream, *a, shift);
+    // 2048 rows or 8192 pages (more than a step changes, unless requests come and go) per workgroup
+    const int64_t rows = a->slot_map ? a->n_rows : 0, pages = (int64_t)a->n_seq * a->table_width;
+    const int64_t grid = (rows + 2047) / 2048 + ((pages < a->n_blocks ? pages : a->n_blocks) >> 13);
+    hipLaunchKernelGGL(paged_plan_kernel, dim3((unsigned)(grid < 1 ? 1 : grid > 256 ? 256 : grid)), dim3(PLAN_NT), lds, (hipStream_t)stream, *a, shift);
     M5_CHECK_LAUNCH();
     return M5_OK;
 }
