@@ -277,31 +277,35 @@ def nar_uniforms(args: L.NarUniformArgs, stream: Optional[int] = None) -> None:
 
 
 # ---- paged serving (include/mars5_paged.h: M5Paged*Args, M5DraftVerifyArgs).  The tensors of a call live on one device, which need not be
-# the current one; `stream` (a raw handle of that device) defaults to torch's current stream there.
-def _launch(fn, what: str, lead: tuple, args, dev: torch.device, stream: Optional[int]) -> None:
-    if dev.index == torch.cuda.current_device():
-        check(fn(*lead, args, torch.cuda.current_stream(dev).cuda_stream if stream is None else stream), what)
-        return
-    with torch.cuda.device(dev):
-        check(fn(*lead, args, torch.cuda.current_stream(dev).cuda_stream if stream is None else stream), what)
+# the current one; `stream` (a raw handle of that device) defaults to torch's current stream there.  A decode step makes dozens of these
+# calls, each of them a few microseconds long on the GPU: the checks are written out inline, without helpers per tensor.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_NO_DEVICE = "libmars5_hip operates on device memory only"
+_DEVICES = "the tensors of a call live on one device"
 
 
-def _same_device(dev: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    assert dev.type == "cuda", "libmars5_hip operates on device memory only"
-    for t in tensors:
-        assert t is None or t.device == dev, f"a tensor is on {t.device}, the call's first one on {dev}"
+def _launch(fn, what: str, lead: tuple, args, idx: int, stream: Optional[int]) -> None:
+    if stream is None:
+        stream = _raw_stream(idx)
+    if idx == torch.cuda.current_device():
+        rc = fn(*lead, args, stream)
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*lead, args, stream)
+    if rc:
+        check(rc, what)
 
 
-def _words(n: int, *tensors: torch.Tensor) -> None:
-    for t in tensors:
-        assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.shape[0] == n, \
-            f"expected {n} contiguous int32 words, got {t.dtype} {tuple(t.shape)}"
-
-
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, n_kv_heads: int, head_dim: int) -> None:
-    for c in (k_cache, v_cache):
-        assert c.dtype == dtype and c.dim() == 4 and c.shape == k_cache.shape and c.stride(3) == 1, "caches: (n_blocks, n_kv_heads, block_size, head_dim)"
-        assert c.shape[1] == n_kv_heads and c.shape[3] == head_dim, f"cache {tuple(c.shape)} for {n_kv_heads} kv heads of {head_dim}"
+def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, n_kv_heads: int, head_dim: int) -> tuple:
+    """(n_blocks, block_size, k pointer and strides, v pointer and strides) of caches (n_blocks, n_kv_heads, block_size, head_dim)."""
+    shape = k_cache.shape
+    assert k_cache.dtype == v_cache.dtype == dtype and v_cache.shape == shape and len(shape) == 4, "caches: (n_blocks, n_kv_heads, block_size, head_dim), the rows' type"
+    assert shape[1] == n_kv_heads and shape[3] == head_dim, f"cache {tuple(shape)} for {n_kv_heads} kv heads of {head_dim}"
+    kb, kh, ks, k1 = k_cache.stride()
+    vb, vh, vs, v1 = v_cache.stride()
+    assert k1 == v1 == 1, "caches: features are contiguous"
+    return shape[0], shape[2], (k_cache.data_ptr(), kb, kh, ks), (v_cache.data_ptr(), vb, vh, vs)
 
 
 def paged_plan(seq_len: torch.Tensor, keep_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
@@ -309,26 +313,29 @@ def paged_plan(seq_len: torch.Tensor, keep_len: torch.Tensor, new_len: torch.Ten
                positions: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
     """One step of a paged cache: request b keeps keep_len[b] of its seq_len[b] positions and adds new_len[b]; block_table
     (n_seq, width), the free stack (free_blocks, state[PST_FREE]) and seq_len are brought up to date, q_start (n_seq + 1,),
-    slot_map and positions (n_rows,) describe the step's rows.  All int32.  state (PST_WORDS,): zero-filled once, then
-    state[PST_FREE] = the number of free ids; state[PST_STATUS] != 0 afterwards: nothing was done (include/mars5_paged.h).  One launch."""
-    dev, B = seq_len.device, seq_len.shape[0]
-    _same_device(dev, keep_len, new_len, block_table, free_blocks, state, q_start, slot_map, positions)
-    _words(B, seq_len, keep_len, new_len)
-    _words(B + 1, q_start)
-    _words(L.PST_WORDS, state)
-    _words(free_blocks.shape[0], free_blocks)
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B and block_table.stride(1) == 1, "block_table: (n_seq, width) int32"
+    slot_map and positions (n_rows,) describe the step's rows (None: not wanted).  All int32.  state (PST_WORDS,): zero-filled once,
+    then state[PST_FREE] = the number of free ids; state[PST_STATUS] != 0 afterwards: nothing was done (include/mars5_paged.h).
+    The tensors must not overlap.  One launch."""
+    idx, (B,), (n_blocks,) = seq_len.get_device(), seq_len.shape, free_blocks.shape
+    assert idx >= 0, _NO_DEVICE
+    assert (idx == keep_len.get_device() == new_len.get_device() == block_table.get_device() == free_blocks.get_device() == state.get_device() ==
+            q_start.get_device()), _DEVICES
+    assert (seq_len.dtype == keep_len.dtype == new_len.dtype == block_table.dtype == free_blocks.dtype == state.dtype == q_start.dtype == _I32), "int32 tensors"
+    assert keep_len.shape == new_len.shape == (B,) and q_start.shape == (B + 1,) and state.shape == (L.PST_WORDS,), "keep_len, new_len (n_seq,), q_start (n_seq + 1,), state (PST_WORDS,)"
+    assert (seq_len.is_contiguous() and keep_len.is_contiguous() and new_len.is_contiguous() and free_blocks.is_contiguous() and state.is_contiguous() and
+            q_start.is_contiguous()), "contiguous tensors (a table's rows may lie apart)"
+    assert block_table.dim() == 2 and block_table.shape[0] == B and block_table.stride(1) == 1, "block_table: (n_seq, width)"
     assert (slot_map is None) == (positions is None), "slot_map and positions go together"
-    n_rows = 0
+    n_rows, slots, where = 0, None, None
     if slot_map is not None:
-        n_rows = slot_map.shape[0]
-        _words(n_rows, slot_map, positions)
-    described = n_rows > 0          # an empty tensor has no address: rows of an empty step are not described
-    assert slot_map is None or described, "slot_map of no rows: pass None"
-    args = L.PagedPlanArgs(seq_len.data_ptr(), keep_len.data_ptr(), new_len.data_ptr(), B, block_table.shape[1], free_blocks.shape[0], block_size, n_rows,
-                           block_table.data_ptr(), block_table.stride(0), free_blocks.data_ptr(), state.data_ptr(), q_start.data_ptr(),
-                           slot_map.data_ptr() if described else None, positions.data_ptr() if described else None)
-    _launch(lib.m5_paged_plan, "m5_paged_plan", (), C.byref(args), dev, stream)
+        (n_rows,) = slot_map.shape
+        assert n_rows > 0, "slot_map of no rows: pass None"
+        assert idx == slot_map.get_device() == positions.get_device(), _DEVICES
+        assert slot_map.dtype == positions.dtype == _I32 and positions.shape == (n_rows,) and slot_map.is_contiguous() and positions.is_contiguous(), "slot_map, positions: (n_rows,) int32"
+        slots, where = slot_map.data_ptr(), positions.data_ptr()
+    args = L.PagedPlanArgs(seq_len.data_ptr(), keep_len.data_ptr(), new_len.data_ptr(), B, block_table.shape[1], n_blocks, block_size, n_rows,
+                           block_table.data_ptr(), block_table.stride(0), free_blocks.data_ptr(), state.data_ptr(), q_start.data_ptr(), slots, where)
+    _launch(lib.m5_paged_plan, "m5_paged_plan", (), C.byref(args), idx, stream)
 
 
 def paged_rope_cache(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rope: torch.Tensor, positions: torch.Tensor, slot_map: torch.Tensor,
@@ -337,44 +344,57 @@ def paged_rope_cache(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rope: tor
     """``rope_cache`` for a paged cache: qkv (n_rows, (n_heads + 2 n_kv_heads) head_dim) -> RMSNorm of every q / k head (weights fp32
     (head_dim,), None = none), rotation by rope (n_pos, n_pairs, 2) fp32 (tables.rope_table) at positions, q -> q_out
     (n_rows, n_heads, head_dim), k / v -> slot_map of the caches (n_blocks, n_kv_heads, block_size, head_dim), any strides with
-    contiguous features.  Rows of slot or position -1 are skipped.  One launch."""
-    dev, (rows, width), hd = qkv.device, qkv.shape, q_out.shape[2]
-    _same_device(dev, rope, positions, slot_map, q_out, k_cache, v_cache, q_norm, k_norm)
-    assert qkv.stride(1) == 1 and width == (n_heads + 2 * n_kv_heads) * hd, f"qkv has {width} columns, {n_heads} + 2 * {n_kv_heads} heads of {hd} need others"
-    assert q_out.dtype == qkv.dtype and q_out.shape == (rows, n_heads, hd) and q_out.stride(2) == 1
-    assert rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous(), "rope: (n_pos, n_pairs, 2) fp32"
-    for w in (q_norm, k_norm):
-        assert w is None or (w.dtype == torch.float32 and w.shape == (hd,) and w.is_contiguous())
-    _words(rows, positions, slot_map)
-    _cache(k_cache, v_cache, qkv.dtype, n_kv_heads, hd)
+    contiguous features.  Rows of slot or position -1 are skipped; slots must be distinct.  One launch."""
+    idx, (rows, width), dt, out_shape = qkv.get_device(), qkv.shape, qkv.dtype, q_out.shape
+    hd = out_shape[2]
+    assert idx >= 0, _NO_DEVICE
+    assert (idx == rope.get_device() == positions.get_device() == slot_map.get_device() == q_out.get_device() == k_cache.get_device() ==
+            v_cache.get_device()), _DEVICES
+    assert width == (n_heads + 2 * n_kv_heads) * hd, f"qkv has {width} columns, {n_heads} + 2 * {n_kv_heads} heads of {hd} need others"
+    assert q_out.dtype == dt and out_shape == (rows, n_heads, hd), "q_out: (n_rows, n_heads, head_dim), qkv's type"
+    assert rope.dtype == _F32 and rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous(), "rope: (n_pos, n_pairs, 2) fp32"
+    assert positions.dtype == slot_map.dtype == _I32 and positions.shape == slot_map.shape == (rows,), "positions, slot_map: (n_rows,) int32"
+    assert positions.is_contiguous() and slot_map.is_contiguous() and qkv.stride(1) == 1
+    q_rs, q_hs, q1 = q_out.stride()
+    assert q1 == 1, "q_out: features are contiguous"
+    n_blocks, block_size, k, v = _caches(k_cache, v_cache, dt, n_kv_heads, hd)
+    qw = kw = None
+    if q_norm is not None:
+        assert q_norm.dtype == _F32 and q_norm.shape == (hd,) and q_norm.is_contiguous() and q_norm.get_device() == idx, "q_norm: (head_dim,) fp32"
+        qw = q_norm.data_ptr()
+    if k_norm is not None:
+        assert k_norm.dtype == _F32 and k_norm.shape == (hd,) and k_norm.is_contiguous() and k_norm.get_device() == idx, "k_norm: (head_dim,) fp32"
+        kw = k_norm.data_ptr()
     if rows == 0:
         return
-    args = L.PagedRopeArgs(qkv.data_ptr(), qkv.stride(0), rows, n_heads, n_kv_heads, hd,
-                           None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-                           rope.data_ptr(), rope.shape[0], rope.shape[1], int(interleaved), positions.data_ptr(), slot_map.data_ptr(),
-                           q_out.data_ptr(), q_out.stride(0), q_out.stride(1), k_cache.data_ptr(), *k_cache.stride()[:3],
-                           v_cache.data_ptr(), *v_cache.stride()[:3], k_cache.shape[0], k_cache.shape[2])
-    _launch(lib.m5_paged_rope_cache, "m5_paged_rope_cache", (DT_CODE[qkv.dtype],), C.byref(args), dev, stream)
+    args = L.PagedRopeArgs(qkv.data_ptr(), qkv.stride(0), rows, n_heads, n_kv_heads, hd, qw, kw, eps, rope.data_ptr(), rope.shape[0], rope.shape[1], interleaved,
+                           positions.data_ptr(), slot_map.data_ptr(), q_out.data_ptr(), q_rs, q_hs, *k, *v, n_blocks, block_size)
+    _launch(lib.m5_paged_rope_cache, "m5_paged_rope_cache", (DT_CODE[dt],), C.byref(args), idx, stream)
 
 
-def _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, scale, window, max_new, workspace) -> L.PagedAttnArgs:
-    dev, B = q.device, seq_len.shape[0]
-    rows, heads, hd = q.shape
-    _same_device(dev, k_cache, v_cache, block_table, seq_len, q_start, out, workspace)
-    assert q.stride(2) == 1 and out.dtype == q.dtype and out.shape == q.shape and out.stride(2) == 1
-    _cache(k_cache, v_cache, q.dtype, k_cache.shape[1], hd)
-    _words(B, seq_len)
-    _words(B + 1, q_start)
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B and block_table.stride(1) == 1, "block_table: (n_seq, width) int32"
-    assert heads % k_cache.shape[1] == 0, f"{heads} query heads over {k_cache.shape[1]} kv heads"
+def _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, scale, window, max_new, workspace) -> tuple:
+    idx, (rows, heads, hd), (B,), dt = q.get_device(), q.shape, seq_len.shape, q.dtype
+    assert idx >= 0, _NO_DEVICE
+    assert (idx == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == seq_len.get_device() == q_start.get_device() ==
+            out.get_device()), _DEVICES
+    assert out.dtype == dt and out.shape == q.shape, "out: q's shape and type"
+    q_rs, q_hs, q1 = q.stride()
+    o_rs, o_hs, o1 = out.stride()
+    assert q1 == o1 == 1, "q, out: features are contiguous"
+    kv = k_cache.shape[1]
+    n_blocks, block_size, k, v = _caches(k_cache, v_cache, dt, kv, hd)
+    assert heads % kv == 0, f"{heads} query heads over {kv} kv heads"
+    assert seq_len.dtype == q_start.dtype == block_table.dtype == _I32 and q_start.shape == (B + 1,) and seq_len.is_contiguous() and q_start.is_contiguous(), \
+        "seq_len (n_seq,), q_start (n_seq + 1,), block_table (n_seq, width): int32"
+    assert block_table.dim() == 2 and block_table.shape[0] == B and block_table.stride(1) == 1, "block_table: (n_seq, width)"
     assert window >= 0 and (scale is None or scale > 0)
+    ws = ws_bytes = 0
     if workspace is not None:
-        assert workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous(), "workspace: zero-filled uint8 bytes"
-    return L.PagedAttnArgs(q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3],
-                           block_table.data_ptr(), block_table.stride(0), block_table.shape[1], k_cache.shape[0], k_cache.shape[2],
-                           B, rows, rows if max_new is None else max_new, heads, k_cache.shape[1], hd, window, seq_len.data_ptr(), q_start.data_ptr(),
-                           hd ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1),
-                           None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.shape[0])
+        assert workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous() and workspace.get_device() == idx, "workspace: zero-filled uint8 bytes"
+        ws, ws_bytes = workspace.data_ptr(), workspace.shape[0]
+    return idx, L.PagedAttnArgs(q.data_ptr(), q_rs, q_hs, *k, *v, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], n_blocks, block_size,
+                                B, rows, rows if max_new is None else max_new, heads, kv, hd, window, seq_len.data_ptr(), q_start.data_ptr(),
+                                hd ** -0.5 if scale is None else scale, out.data_ptr(), o_rs, o_hs, ws, ws_bytes)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor,
@@ -383,17 +403,18 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """out (n_rows, n_heads, head_dim) = causal attention of every request's new rows q over its seq_len[b] cached positions (the
     rows' own included), optionally through a sliding window.  Rows from q_start[-1] on are padding.  scale: 1 / sqrt(head_dim).
     max_new: upper bound of the new tokens of one request (speed only).  workspace: uint8, zero-filled once, one for every call
-    that may be in flight at a time; without it keys are not split over workgroups (paged_attention_workspace: how much)."""
+    that may be in flight at a time; without it keys are not split over workgroups (paged_attention_workspace: how much).
+    One launch."""
     if q.shape[0] == 0:
         return
-    args = _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, scale, window, max_new, workspace)
-    _launch(lib.m5_paged_attention, "m5_paged_attention", (DT_CODE[q.dtype],), C.byref(args), q.device, stream)
+    idx, args = _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, scale, window, max_new, workspace)
+    _launch(lib.m5_paged_attention, "m5_paged_attention", (DT_CODE[q.dtype],), C.byref(args), idx, stream)
 
 
 def paged_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor,
                               q_start: torch.Tensor, out: torch.Tensor, window: int = 0, max_new: Optional[int] = None) -> int:
     """Bytes of workspace that paged_attention can use for tensors of these shapes (it works with fewer)."""
-    args = _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, None, window, max_new, None)
+    _, args = _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, None, window, max_new, None)
     n = L.i64(0)
     check(lib.m5_paged_attention_workspace(DT_CODE[q.dtype], C.byref(args), C.byref(n)), "m5_paged_attention_workspace")
     return int(n.value)
@@ -407,27 +428,31 @@ def draft_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: to
     fp32 (U[0, 1) and Exp(1)).  out_tokens (n_seq, width) int64 = accepted drafts, one drawn token, -1; n_out (n_seq,) int32;
     keep_len = seq_len - rows + n_out for the next paged_plan.  workspace: DRAFT_WS_BYTES per request (uint8, zero-filled once, one
     for every call that may be in flight at a time), or None.  One launch."""
-    dev, (rows, V), B = target.device, target.shape, n_out.shape[0]
-    _same_device(dev, draft, tokens, row_start, uniforms, noise, out_tokens, n_out, seq_len, keep_len, workspace)
-    assert rows > 0 and target.stride(1) == 1
-    assert draft is None or (draft.shape == target.shape and draft.dtype == target.dtype and draft.stride(1) == 1)
-    assert tokens.dtype == torch.int64 and tokens.shape == (rows,) and tokens.is_contiguous()
-    assert uniforms.dtype == torch.float32 and uniforms.shape == (rows,) and uniforms.is_contiguous()
-    assert noise.dtype == torch.float32 and noise.shape == (B, V) and noise.stride(1) == 1
-    assert out_tokens.dtype == torch.int64 and out_tokens.dim() == 2 and out_tokens.shape[0] == B and out_tokens.stride(1) == 1
+    idx, (rows, V), (B,), dt = target.get_device(), target.shape, n_out.shape, target.dtype
+    assert idx >= 0, _NO_DEVICE
+    assert (idx == tokens.get_device() == row_start.get_device() == uniforms.get_device() == noise.get_device() == out_tokens.get_device() ==
+            n_out.get_device()), _DEVICES
+    assert rows > 0 and target.stride(1) == 1, "target: (n_rows, vocab)"
+    assert tokens.dtype == _I64 and tokens.shape == (rows,) and tokens.is_contiguous(), "tokens: (n_rows,) int64"
+    assert uniforms.dtype == noise.dtype == _F32 and uniforms.shape == (rows,) and uniforms.is_contiguous() and noise.shape == (B, V) and noise.stride(1) == 1, \
+        "uniforms (n_rows,), noise (n_seq, vocab): fp32"
+    assert out_tokens.dtype == _I64 and out_tokens.dim() == 2 and out_tokens.shape[0] == B and out_tokens.stride(1) == 1, "out_tokens: (n_seq, width) int64"
+    assert row_start.dtype == n_out.dtype == _I32 and row_start.shape == (B + 1,) and row_start.is_contiguous() and n_out.is_contiguous(), "row_start (n_seq + 1,), n_out (n_seq,): int32"
     assert (seq_len is None) == (keep_len is None), "seq_len and keep_len go together"
-    _words(B + 1, row_start)
-    _words(B, n_out)
+    q = q_rs = held = kept = ws = ws_bytes = 0
+    if draft is not None:
+        assert draft.shape == target.shape and draft.dtype == dt and draft.stride(1) == 1 and draft.get_device() == idx, "draft: target's shape and type"
+        q, q_rs = draft.data_ptr(), draft.stride(0)
     if seq_len is not None:
-        _words(B, seq_len, keep_len)
+        assert idx == seq_len.get_device() == keep_len.get_device(), _DEVICES
+        assert seq_len.dtype == keep_len.dtype == _I32 and seq_len.shape == keep_len.shape == (B,) and seq_len.is_contiguous() and keep_len.is_contiguous(), "seq_len, keep_len: (n_seq,) int32"
+        held, kept = seq_len.data_ptr(), keep_len.data_ptr()
     if workspace is not None:
-        assert workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous(), "workspace: zero-filled uint8 bytes"
-    args = L.DraftVerifyArgs(target.data_ptr(), target.stride(0), None if draft is None else draft.data_ptr(), 0 if draft is None else draft.stride(0),
-                             rows, V, B, out_tokens.shape[1], tokens.data_ptr(), row_start.data_ptr(), uniforms.data_ptr(), noise.data_ptr(), noise.stride(0),
-                             out_tokens.data_ptr(), out_tokens.stride(0), n_out.data_ptr(), None if seq_len is None else seq_len.data_ptr(),
-                             None if keep_len is None else keep_len.data_ptr(), None if workspace is None else workspace.data_ptr(),
-                             0 if workspace is None else workspace.shape[0])
-    _launch(lib.m5_draft_verify, "m5_draft_verify", (DT_CODE[target.dtype],), C.byref(args), dev, stream)
+        assert workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous() and workspace.get_device() == idx, "workspace: zero-filled uint8 bytes"
+        ws, ws_bytes = workspace.data_ptr(), workspace.shape[0]
+    args = L.DraftVerifyArgs(target.data_ptr(), target.stride(0), q, q_rs, rows, V, B, out_tokens.shape[1], tokens.data_ptr(), row_start.data_ptr(), uniforms.data_ptr(),
+                             noise.data_ptr(), noise.stride(0), out_tokens.data_ptr(), out_tokens.stride(0), n_out.data_ptr(), held, kept, ws, ws_bytes)
+    _launch(lib.m5_draft_verify, "m5_draft_verify", (DT_CODE[dt],), C.byref(args), idx, stream)
 
 
 def expand_tokens(tokens: torch.Tensor, n_text: int, off: torch.Tensor, vals: torch.Tensor, max_run: int,
