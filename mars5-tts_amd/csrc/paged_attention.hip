@@ -25,6 +25,7 @@
 #include "common.h"
 #include "paged_index.h"
 #include <limits.h>
+#include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) _Float16 h8_t;
 typedef __attribute__((ext_vector_type(8))) __bf16 b8_t;
@@ -36,25 +37,42 @@ namespace {
 
 constexpr int NWAVE = 4, NT = NWAVE * 64;
 constexpr int MAXP = 1024;                       // block ids of one key segment held in LDS
+constexpr int MAX_SLOTS = 4096;                  // partial results of a call, and their bytes
+constexpr int64_t MAX_SLOT_BYTES = 64 << 20;
+constexpr int MIN_UNITS = 8;                     // shortest chunk of keys, in 64s: joining costs about as much as 600 keys (5 short requests: 8.2 us; 10.2 with 4)
 constexpr int MAX_SEQ = 4096;                    // item prefix sums in LDS: 16 KB
 constexpr int IDS_B = MAXP * 4, ML_B = NWAVE * 64 * 2 * 4 + 64;
 constexpr int odd_bytes(int hd) { return NWAVE * 2 * hd * 4; }   // notes of non-finite values: per wave and feature 2 x 32 keys, or 2 x 64 shared
 
+// x / d for 0 <= x < 2^29: (x m) >> s with m = ceil(2^s / d), s = 29 + ceil(log2 d)
+struct Div {
+    uint32_t d, m, s;
+    void set(int by) {
+        d = (uint32_t)by;
+        s = 29;
+        while ((1u << (s - 29)) < d) ++s;
+        m = (uint32_t)((((uint64_t)1 << s) + d - 1) / d);
+    }
+    __device__ inline int div(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> s); }
+};
+
 struct Launch {
     M5PagedAttnArgs a;
-    int shift, group;
-    int target;                                  // items wanted: places on the chip
-    int n_slots;                                 // partial results the workspace holds, 0 = keys are not split
+    int shift;
+    Div group, kv;                               // query heads of a kv head; kv heads
+    int places;                                  // workgroups that the chip holds at a time
+    int n_big, n_few;                            // partial results of the largest / of few-row tiles that the workspace holds (0: keys are not split)
     float* slots; int* tickets;
-    int64_t slot_floats;                         // floats of one partial result: rows of o, then (m, l) per row
     float sc2;                                   // scale * log2(e)
 };
 
 struct Item {
     M5Request rq;
-    int b, kvh, rows, rho0, rho1;                // rows of the request's kv head, [rho0, rho1) of them here
+    int b, kvh, rho0, rho1;                      // packed rows of the request and kv head
     int ka, kb;                                  // keys of this item
-    int id, first_id, n_parts;                   // partial results of this tile: slots first_id + p * n_kv_heads
+    int n_parts;                                 // partial results of this tile; more than one: this item's goes to `slot`, the tile's
+    float* slot; float* first_slot;              // lie part_stride floats apart from first_slot on, and meet at `ticket`
+    int64_t part_stride; int* ticket;
 };
 
 // ---------------------------------------------------------------------------------------------------- small pieces
@@ -69,6 +87,13 @@ __device__ inline f4_t mma16(const uint4& a, const uint4& b, f4_t c, F32T) {    
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
     return c;
+}
+typedef __attribute__((ext_vector_type(4))) _Float16 h4_t;
+__device__ inline f4_t mma16(const uint2& a, const uint2& b, f4_t c, F16T) {      // 16 keys: half a fragment
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(*reinterpret_cast<const h4_t*>(&a), *reinterpret_cast<const h4_t*>(&b), c, 0, 0, 0);
+}
+__device__ inline f4_t mma16(const uint2& a, const uint2& b, f4_t c, BF16T) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(*reinterpret_cast<const s4_t*>(&a), *reinterpret_cast<const s4_t*>(&b), c, 0, 0, 0);
 }
 __device__ inline f16_t mma32(const uint4& a, const uint4& b, f16_t c, F16T) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8_t*>(&a), *reinterpret_cast<const h8_t*>(&b), c, 0, 0, 0);
@@ -134,6 +159,18 @@ __device__ inline int key_block(const int* ids, int page0, int key, int ka, int 
     return key >= ka && key < kb ? ids[(key >> shift) - page0] : -1;
 }
 
+// Partial results cross between workgroups (and XCDs, whose L2s do not share lines) as agent-scope accesses: written through to memory and
+// read from there.  A workgroup's stores are waited for before its ticket is drawn, so no cache has to be written back or invalidated
+// (an acquire-release ticket does both for the whole L2: 64 requests of 1 to 16 thousand keys 380 us instead of 328).
+__device__ inline void put_part(float* p, float a, float b) {
+    __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), (unsigned long long)__float_as_uint(a) | (unsigned long long)__float_as_uint(b) << 32,
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float2 get_part(const float* p) {
+    const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
 // softmax state of one row block: new maximum from this lane's scores (already reduced over the lanes of the row)
 struct Soft {
     float m, l;
@@ -152,8 +189,8 @@ __device__ inline void put_row(const Launch& L, const Item& it, int row, int d, 
     const int rho = it.rho0 + row;
     if (it.n_parts <= 1) {
         const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);         // (NaN stays NaN)
-        typename T::storage* out = (typename T::storage*)L.a.out + (int64_t)(it.rq.r0 + rho / L.group) * L.a.o_rs +
-                                   (int64_t)(it.kvh * L.group + rho % L.group) * L.a.o_hs + d;
+        typename T::storage* out = (typename T::storage*)L.a.out + (int64_t)(it.rq.r0 + L.group.div(rho)) * L.a.o_rs +
+                                   (int64_t)(it.kvh * L.group.d + rho - L.group.div(rho) * L.group.d) * L.a.o_hs + d;
         if (l == 0.f) o = f4_t{0.f, 0.f, 0.f, 0.f};
         if constexpr (T::EPL == 4) *reinterpret_cast<f4_t*>(out) = o * inv;
         else *reinterpret_cast<uint2*>(out) = m5_pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
@@ -161,16 +198,20 @@ __device__ inline void put_row(const Launch& L, const Item& it, int row, int d, 
 }
 
 // ------------------------------------------------------------------------------------------------------ few rows
-template <typename T, int HD, int R, int NW>
+template <typename T, int HD, int R>
 struct Few {
     using st = typename T::storage;
     static constexpr int ES = sizeof(st), RB = HD * ES;          // bytes of a row
-    static constexpr int KS = ES == 4 ? 16 : 32, SUB = KS / 16;  // keys of a stage
+    // Keys of a stage: 8 KB of K and V, so that two workgroups share a CU and one computes while the other starts or ends an item (one
+    // workgroup of 16 KB stages: decode_long 178 us when its items filled the chip exactly once, 211-257 in 2-4 rounds).  Not for
+    // 64 rows of 128 features (their registers allow one workgroup anyway) and fp32 (16 KB).
+    static constexpr int KS = ES == 4 || (HD == 128 && R < 4) ? 16 : 32, SUB = KS / 16;
+    using Frag = std::conditional_t<ES == 2 && SUB == 1, uint2, uint4>;      // a lane's keys of the second product
     static constexpr int LPR = RB / 16, RPI = 64 / LPR;          // lanes per row, rows per DMA instruction
     static constexpr int NI = KS / RPI;                          // DMA instructions of K (and of V) per stage
     static constexpr int OP_B = KS * RB, STAGE_B = 2 * OP_B, WAVE_B = 2 * STAGE_B;
     static constexpr int NF = RB / 64, ND = HD / 16;             // K fragments per key row block, feature blocks of V
-    static constexpr int LDS_B = NW * WAVE_B;
+    static constexpr int LDS_B = NWAVE * WAVE_B;
     static_assert(R * 16 * HD * 4 <= WAVE_B, "the waves' results meet in their rings");
 
     // 16-byte chunk swizzles: 16 (8 for V) rows of one chunk column fall into different banks
@@ -214,13 +255,13 @@ struct Few {
         int qpos[R];
 #pragma unroll
         for (int rb = 0; rb < R; ++rb) {
-            const int rho = min(it.rho0 + rb * 16 + c, it.rho1 - 1), tok = rho / L.group;
+            const int rho = min(it.rho0 + rb * 16 + c, it.rho1 - 1), tok = L.group.div(rho);
             qpos[rb] = pos0 + tok;
-            const st* q = (const st*)p.q + (int64_t)(it.rq.r0 + tok) * p.q_rs + (int64_t)(it.kvh * L.group + rho % L.group) * p.q_hs;
+            const st* q = (const st*)p.q + (int64_t)(it.rq.r0 + tok) * p.q_rs + (int64_t)(it.kvh * L.group.d + rho - tok * L.group.d) * p.q_hs;
 #pragma unroll
             for (int t = 0; t < NF; ++t) qf[rb][t] = *reinterpret_cast<const uint4*>(q + (4 * t + g) * T::EPL);
         }
-        const int pos_min = pos0 + it.rho0 / L.group, pos_max = pos0 + (it.rho1 - 1) / L.group;
+        const int pos_min = pos0 + L.group.div(it.rho0), pos_max = pos0 + L.group.div(it.rho1 - 1);
         const int lo_max = m5_key_lo(pos_max, p.window);         // the last row's first key
         f4_t o[R][ND];
         Soft sm[R];
@@ -237,7 +278,7 @@ struct Few {
         const unsigned char* Kg = (const unsigned char*)p.k_cache + (int64_t)it.kvh * p.k_hs * ES;
         const unsigned char* Vg = (const unsigned char*)p.v_cache + (int64_t)it.kvh * p.v_hs * ES;
         const int off_mask = (1 << L.shift) - 1;
-        const int step = NW * KS;                                // keys of one round of the waves
+        const int step = NWAVE * KS;                                // keys of one round of the waves
         const int64_t seg = ((int64_t)(MAXP - 1) << L.shift) / step * step;
         const int k_first = it.ka & ~(KS - 1);
 
@@ -248,7 +289,6 @@ struct Few {
             __syncthreads();
             for (int i = tid; i < np; i += NT) ids[i] = m5_block(p.block_table[(int64_t)it.b * p.table_rs + page0 + i], p.n_blocks);
             __syncthreads();
-            if (wave >= NW) continue;
             auto fetch = [&](int kb, int stage) {
                 const uint32_t to = ring + stage * STAGE_B;
 #pragma unroll
@@ -281,7 +321,7 @@ struct Few {
                             if (R == 1 || rb < nrb) s[rb][h] = mma16(k, qf[rb][t], s[rb][h], T());
                     }
                 }
-                uint4 pf[R];
+                Frag pf[R];
 #pragma unroll
                 for (int rb = 0; rb < R; ++rb) {
                     if (R > 1 && rb >= nrb) continue;
@@ -302,7 +342,7 @@ struct Few {
                     float use;
                     const float alpha = sm[rb].step(mx, use);
                     float sum = 0.f;
-                    st e[T::EPL];
+                    __attribute__((aligned(16))) st e[4 * SUB];
 #pragma unroll
                     for (int h = 0; h < SUB; ++h)
 #pragma unroll
@@ -311,7 +351,7 @@ struct Few {
                             sum += x;
                             e[4 * h + r] = T::from_f32(x);       // 16-bit: p in (0, 1] rounded once for the matrix product, summed in fp32
                         }
-                    pf[rb] = *reinterpret_cast<const uint4*>(e);
+                    pf[rb] = *reinterpret_cast<const Frag*>(e);
                     sm[rb].l = sm[rb].l * alpha + sum;
                     if (!__all(alpha == 1.0f))
 #pragma unroll
@@ -319,7 +359,7 @@ struct Few {
                 }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    uint4 v;
+                    Frag v;
                     if constexpr (ES == 4) {
                         uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
@@ -328,13 +368,14 @@ struct Few {
                             w[r] = *reinterpret_cast<const uint32_t*>(vs + row * RB + (((4 * d + (c >> 2)) ^ vswz(row)) << 4) + (c & 3) * 4);
                         }
                     } else {
-                        uint2 h2[2];
+                        uint2 half[SUB];
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
+                        for (int h = 0; h < SUB; ++h) {
                             const int row = 16 * h + 4 * g + (c >> 2);
-                            h2[h] = tr_read(vs + row * RB + (((2 * d + ((c >> 1) & 1)) ^ vswz(row)) << 4) + (c & 1) * 8);
+                            half[h] = tr_read(vs + row * RB + (((2 * d + ((c >> 1) & 1)) ^ vswz(row)) << 4) + (c & 1) * 8);
                         }
-                        v = make_uint4(h2[0].x, h2[0].y, h2[1].x, h2[1].y);
+                        if constexpr (SUB == 2) v = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
+                        else v = half[0];
                     }
 #pragma unroll
                     for (int rb = 0; rb < R; ++rb)
@@ -369,38 +410,37 @@ struct Few {
         // ---- the waves' results meet: row-major fp32 in the rings, chunk-swizzled
         __syncthreads();
         float* om = reinterpret_cast<float*>(mine);
-        if (wave < NW) {
 #pragma unroll
-            for (int rb = 0; rb < R; ++rb) {
-                if (R > 1 && rb >= nrb) continue;
-                float l = sm[rb].l;
-                l += lane_xor16(l);
-                l += lane_xor32(l);
-                const int row = rb * 16 + c;
-                if (g == 0) { ml[(wave * 64 + row) * 2] = sm[rb].m; ml[(wave * 64 + row) * 2 + 1] = l; }
+        for (int rb = 0; rb < R; ++rb) {
+            if (R > 1 && rb >= nrb) continue;
+            float l = sm[rb].l;
+            l += lane_xor16(l);
+            l += lane_xor32(l);
+            const int row = rb * 16 + c;
+            if (g == 0) { ml[(wave * 64 + row) * 2] = sm[rb].m; ml[(wave * 64 + row) * 2 + 1] = l; }
 #pragma unroll
-                for (int d = 0; d < ND; ++d) *reinterpret_cast<f4_t*>(om + row * HD + (((4 * d + g) ^ (row & 15)) << 2)) = o[rb][d];
-            }
+            for (int d = 0; d < ND; ++d) *reinterpret_cast<f4_t*>(om + row * HD + (((4 * d + g) ^ (row & 15)) << 2)) = o[rb][d];
         }
         __syncthreads();
-        float* slot = it.n_parts > 1 ? L.slots + it.id * L.slot_floats : nullptr;
+        float* slot = it.n_parts > 1 ? it.slot : nullptr;
         const int chunks = (it.rho1 - it.rho0) * (HD / 4);
         for (int i = tid; i < chunks; i += NT) {
             const int row = i / (HD / 4), ch = i % (HD / 4);
             float m = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[(w * 64 + row) * 2]);
+            for (int w = 0; w < NWAVE; ++w) m = fmaxf(m, ml[(w * 64 + row) * 2]);
             const float use = m == -INFINITY ? 0.f : m;
             f4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
+            for (int w = 0; w < NWAVE; ++w) {
                 const float f = __builtin_amdgcn_exp2f(ml[(w * 64 + row) * 2] - use);
                 l += ml[(w * 64 + row) * 2 + 1] * f;
                 sum += *reinterpret_cast<const f4_t*>(reinterpret_cast<const float*>(lds + w * WAVE_B) + row * HD + ((ch ^ (row & 15)) << 2)) * f;
             }
             if (slot) {
-                *reinterpret_cast<f4_t*>(slot + row * HD + ch * 4) = sum;
-                if (ch == 0) { slot[16 * R * HD + 2 * row] = m; slot[16 * R * HD + 2 * row + 1] = l; }
+                put_part(slot + row * HD + ch * 4, sum[0], sum[1]);
+                put_part(slot + row * HD + ch * 4 + 2, sum[2], sum[3]);
+                if (ch == 0) put_part(slot + 16 * R * HD + 2 * row, m, l);
             } else {
                 put_row<T, HD>(L, it, row, ch * 4, sum, m, l);
             }
@@ -454,12 +494,12 @@ struct Many {
         const int c = lane & 31, hh = lane >> 5;
         const int w0 = it.rho0 + wave * 32, w1 = min(w0 + 32, it.rho1);      // this wave's rows (none: it only fetches)
         const int pos0 = it.rq.len - (it.rq.r1 - it.rq.r0);
-        const int rho = min(w0 + c, it.rho1 - 1), tok = rho / L.group, qpos = pos0 + tok;
-        const int pos_min = pos0 + w0 / L.group, pos_max = pos0 + (w1 - 1) / L.group;
+        const int rho = min(w0 + c, it.rho1 - 1), tok = L.group.div(rho), qpos = pos0 + tok;
+        const int pos_min = pos0 + L.group.div(w0), pos_max = pos0 + L.group.div(max(w1 - 1, 0));
         const int lo_min = m5_key_lo(pos_min, p.window), lo_max = m5_key_lo(pos_max, p.window), lo = m5_key_lo(qpos, p.window);
         uint4 qf[NF];
         {
-            const st* q = (const st*)p.q + (int64_t)(it.rq.r0 + tok) * p.q_rs + (int64_t)(it.kvh * L.group + rho % L.group) * p.q_hs;
+            const st* q = (const st*)p.q + (int64_t)(it.rq.r0 + tok) * p.q_rs + (int64_t)(it.kvh * L.group.d + rho - tok * L.group.d) * p.q_hs;
 #pragma unroll
             for (int t = 0; t < NF; ++t) qf[t] = *reinterpret_cast<const uint4*>(q + 16 * t + 8 * hh);
         }
@@ -472,7 +512,7 @@ struct Many {
         const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
         unsigned long long* up = reinterpret_cast<unsigned long long*>(odd_lds);
         unsigned long long* down = up + HD;
-        const int first_pos = pos0 + it.rho0 / L.group, last_lo = m5_key_lo(pos0 + (it.rho1 - 1) / L.group, p.window);      // of all rows here
+        const int first_pos = pos0 + L.group.div(it.rho0), last_lo = m5_key_lo(pos0 + L.group.div(it.rho1 - 1), p.window);      // of all rows here
         const unsigned char* Kg = (const unsigned char*)p.k_cache + (int64_t)it.kvh * p.k_hs * 2;
         const unsigned char* Vg = (const unsigned char*)p.v_cache + (int64_t)it.kvh * p.v_hs * 2;
         const int off_mask = (1 << L.shift) - 1;
@@ -581,180 +621,291 @@ struct Many {
         float l = sm.l + lane_xor32(sm.l);
         if (w0 + c >= w1) return;
         const int row = wave * 32 + c;
-        float* slot = it.n_parts > 1 ? L.slots + it.id * L.slot_floats : nullptr;
-        if (slot && hh == 0) { slot[128 * HD + 2 * row] = sm.m; slot[128 * HD + 2 * row + 1] = l; }
+        float* slot = it.n_parts > 1 ? it.slot : nullptr;
+        if (slot && hh == 0) put_part(slot + 128 * HD + 2 * row, sm.m, l);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const f4_t v = {o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
                 const int at = 32 * d + 8 * q + 4 * hh;
-                if (slot) *reinterpret_cast<f4_t*>(slot + row * HD + at) = v;
-                else put_row<T, HD>(L, it, row, at, v, sm.m, l);
+                if (slot) {
+                    put_part(slot + row * HD + at, v[0], v[1]);
+                    put_part(slot + row * HD + at + 2, v[2], v[3]);
+                } else put_row<T, HD>(L, it, row, at, v, sm.m, l);
             }
     }
 };
 
-// The last workgroup of a tile joins its partial results in chunk order.
+// The last workgroup of a tile joins its partial results: the parts are dealt to groups of threads (one thread holds four features of
+// a row), eight of them in flight per thread, and the groups meet in LDS.  The order depends on the counts alone.
 template <typename T, int HD, int TR>
-__device__ void join_parts(const Launch& L, const Item& it, int* sh_last) {
-    __syncthreads();
+__device__ void join_parts(const Launch& L, const Item& it, unsigned char* lds, int* sh_last) {
+    vm_wait<0>();                                            // this thread's part is in memory,
+    __syncthreads();                                         // and so is the whole workgroup's
     if (threadIdx.x == 0) {
-        int* ticket = L.tickets + it.first_id;
-        const int n = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        int* ticket = it.ticket;
+        const int n = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *sh_last = n == it.n_parts - 1;
         if (n == it.n_parts - 1) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);       // ready for the next call
     }
     __syncthreads();
     if (!*sh_last) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    const float* first = L.slots + it.first_id * L.slot_floats;
-    const int64_t stride = L.a.n_kv_heads * L.slot_floats;
+    const float* first = it.first_slot;
+    const int64_t stride = it.part_stride;
     Item whole = it;
     whole.n_parts = 1;
-    const int chunks = (it.rho1 - it.rho0) * (HD / 4);
-    for (int i = threadIdx.x; i < chunks; i += NT) {
-        const int row = i / (HD / 4), ch = i % (HD / 4);
+    constexpr int C4 = HD / 4, U = 8;
+    const int chunks = (it.rho1 - it.rho0) * C4, groups = chunks < NT ? min(NT / chunks, it.n_parts) : 1;
+    f4_t* meet = reinterpret_cast<f4_t*>(lds);               // [NT] sums, then [NT] (m, l)
+    float2* meet_ml = reinterpret_cast<float2*>(lds + NT * 16);
+    for (int base = 0; base < chunks; base += NT) {
+        const int at = base + (int)threadIdx.x, grp = chunks < NT ? at / chunks : 0, i = chunks < NT ? at - grp * chunks : at;
+        const bool live = grp < groups && i < chunks;
+        const int row = i / C4, ch = i % C4;
         float m = -INFINITY, l = 0.f;
-        for (int k = 0; k < it.n_parts; ++k) m = fmaxf(m, first[k * stride + TR * HD + 2 * row]);
-        const float use = m == -INFINITY ? 0.f : m;
         f4_t sum = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < it.n_parts; ++k) {
-            const float* s = first + k * stride;
-            const float f = __builtin_amdgcn_exp2f(s[TR * HD + 2 * row] - use);
-            l += s[TR * HD + 2 * row + 1] * f;
-            sum += *reinterpret_cast<const f4_t*>(s + row * HD + ch * 4) * f;
+        if (live)
+            for (int k0 = grp; k0 < it.n_parts; k0 += groups * U) {
+                float2 ml[U];
+                f4_t v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = min(k0 + u * groups, it.n_parts - 1);
+                    const float* s = first + k * stride;
+                    ml[u] = get_part(s + TR * HD + 2 * row);
+                    const float2 a = get_part(s + row * HD + ch * 4), b = get_part(s + row * HD + ch * 4 + 2);
+                    v[u] = f4_t{a.x, a.y, b.x, b.y};
+                }
+                float mn = m;
+#pragma unroll
+                for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+                const float use = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - use);
+                m = mn;
+                l *= alpha;
+                sum *= alpha;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float f = k0 + u * groups < it.n_parts ? __builtin_amdgcn_exp2f(ml[u].x - use) : 0.f;
+                    if (f != 0.f) {                          // (a part without weight adds nothing, whatever it holds)
+                        l += ml[u].y * f;
+                        sum += v[u] * f;
+                    }
+                }
+            }
+        if (groups > 1) {
+            meet[threadIdx.x] = sum;
+            meet_ml[threadIdx.x] = make_float2(m, l);
+            __syncthreads();
+            if (grp == 0) {
+                float mn = m;
+                for (int g = 1; g < groups; ++g) mn = fmaxf(mn, meet_ml[g * chunks + i].x);
+                const float use = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - use);
+                l *= alpha;
+                sum *= alpha;
+                for (int g = 1; g < groups; ++g) {
+                    const float2 o = meet_ml[g * chunks + i];
+                    const float f = __builtin_amdgcn_exp2f(o.x - use);
+                    l += o.y * f;
+                    sum += meet[g * chunks + i] * f;
+                }
+                m = mn;
+            }
         }
-        put_row<T, HD>(L, whole, row, ch * 4, sum, m, l);
+        if (live && grp == 0) put_row<T, HD>(L, whole, row, ch * 4, sum, m, l);
     }
 }
 
-__device__ inline int64_t block_sum64(int64_t v, int64_t* red) {             // red: NWAVE words
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor((long long)v, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    int64_t t = 0;
-    for (int w = 0; w < NWAVE; ++w) t += red[w];
-    return t;
+// inclusive sum over the lanes of a wave: DPP row shifts, then the rows' last lanes broadcast
+template <int CTRL, int ROWS>
+__device__ inline int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ inline int wave_scan(int v) {
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    return dpp_add<0x143, 0xc>(v);
 }
 
-// A request's share of the work: tiles of `tr` rows and the keys that any of its rows sees, from k0 (a multiple of 64) on.
-struct Share { int rows, tr, tiles, k0, keys; };
+// A request's share of the work: tiles of `tr` rows and the keys that any of its rows sees, from k0 (a multiple of 64) on, in
+// units of 64.
+struct Share { int rows, tr, tiles, k0, units; };
 template <int TR_FEW, int TR_MANY>
 __device__ inline Share share_of(const Launch& L, const M5Request& rq) {
     Share s;
-    s.rows = (rq.r1 - rq.r0) * L.group;
+    s.rows = (rq.r1 - rq.r0) * (int)L.group.d;
     s.tr = TR_MANY && s.rows > TR_FEW ? TR_MANY : TR_FEW;
-    s.tiles = (s.rows + s.tr - 1) / s.tr;
+    s.tiles = (s.rows + s.tr - 1) / s.tr;                    // (powers of two)
     s.k0 = m5_key_lo(rq.len - (rq.r1 - rq.r0), L.a.window) & ~63;
-    s.keys = max(rq.len - s.k0, 0);
+    s.units = (max(rq.len - s.k0, 0) + 63) >> 6;
     return s;
 }
 
-// R: row blocks of the few-row tiles; NW: waves that work on them; MANY: requests of more rows get 128-row tiles.
-template <typename T, int HD, int R, int NW, bool MANY>
+// Items: every (request, tile, chunk of `cu` units, kv head), numbered by request.  Up to 64 requests a wave keeps in its lanes, more lie
+// in LDS as prefix sums.
+template <int TR_FEW, int TR_MANY, int HD>
+struct Deal {
+    int cu, total;
+    M5Request mine;
+    int incl;
+
+    static constexpr bool MANY = TR_MANY != 0;
+    int slot_rows;                                           // rows that a slot has room for
+
+    __device__ inline int chunks(const Share& s) const {
+        if (s.units <= cu || (MANY && s.tr > slot_rows)) return 1;
+        return (int)((uint32_t)(s.units + cu - 1) / (uint32_t)cu);
+    }
+    // How long a chunk is.  items <= units / cu + tiles, and each needs a slot.
+    //  - Few tiles (at most a quarter of the places): chunks as long as the places, once filled, allow (3 requests of 60 to 120 thousand keys:
+    //    159 us in 512 items, 165 / 175 / 177 in 1024 / 1536 / 2048).
+    //  - Up to two per place: four items per place, so that requests of different lengths end together (64 requests of 1 to 16 thousand
+    //    keys in 512 tiles: 485 us unsplit, 395 / 346 / 328 us in about 850 / 1300 / 1700 items).
+    //  - More balance by themselves, only much longer ones are split (40 requests of 300 to 3000 keys beside a chunk, 1152 tiles: 120 us
+    //    unsplit, 147 with the longer third in two parts).
+    //  - 128-row tiles are split only while slots of their size suffice for all.
+    __device__ inline void length(const Launch& L, float units, float tiles) {
+        units *= (float)L.kv.d;
+        tiles *= (float)L.kv.d;                              // (floats: exact as far as tiles are few enough to be split)
+        const float P = (float)L.places;
+        slot_rows = MANY && tiles < (float)L.n_big ? TR_MANY : TR_FEW;
+        const float slots = (float)(MANY && slot_rows == TR_MANY ? L.n_big : L.n_few);
+        cu = INT_MAX >> 7;
+        if (tiles < slots) {
+            const float room = min(4.f * tiles <= P ? P - tiles : (tiles <= 2.f * P ? 4.f * P - tiles : 0.5f * P), slots - tiles);
+            const float len = max(units * 1.0001f / room + 1.f, units / (128.f * max(tiles, 1.f)));      // at most about 128 parts to a tile
+            cu = (int)min(max(len, (float)MIN_UNITS), (float)(INT_MAX >> 7));
+        }
+    }
+    __device__ inline M5Request request(const Launch& L, int b) const {
+        return m5_request(L.a.q_start[b], L.a.q_start[b + 1], L.a.seq_len[b], L.a.n_rows, (int64_t)L.a.table_width << L.shift);
+    }
+    __device__ void setup(const Launch& L, int* pre, float* red, int* sums) {
+        const int B = L.a.n_seq, tid = threadIdx.x, lane = tid & 63;
+        if (B <= 64) {
+            mine = lane < B ? request(L, lane) : M5Request{0, 0, 0};
+            const Share s = share_of<TR_FEW, TR_MANY>(L, mine);
+            length(L, wave_sum((float)s.tiles * (float)s.units), wave_sum((float)s.tiles));
+            incl = wave_scan(s.tiles * chunks(s) * (int)L.kv.d);
+            total = __builtin_amdgcn_readlane(incl, 63);
+            return;
+        }
+        const int per = (B + NT - 1) / NT, b0 = min(tid * per, B), b1 = min(b0 + per, B);
+        float units = 0.f, tiles = 0.f;
+        for (int b = b0; b < b1; ++b) {
+            const Share s = share_of<TR_FEW, TR_MANY>(L, request(L, b));
+            units += (float)s.tiles * (float)s.units;
+            tiles += (float)s.tiles;
+        }
+        units = block_sum<NWAVE>(units, red);
+        tiles = block_sum<NWAVE>(tiles, red);
+        length(L, units, tiles);
+        int n = 0;
+        for (int b = b0; b < b1; ++b) {
+            const Share s = share_of<TR_FEW, TR_MANY>(L, request(L, b));
+            n += s.tiles * chunks(s) * (int)L.kv.d;
+        }
+        const int upto = wave_scan(n);
+        if (lane == 63) sums[tid >> 6] = upto;
+        __syncthreads();
+        int base = upto - n;
+        total = 0;
+        for (int w = 0; w < NWAVE; ++w) {
+            if (w < tid >> 6) base += sums[w];
+            total += sums[w];
+        }
+        for (int b = b0; b < b1; ++b) {
+            pre[b] = base;
+            const Share s = share_of<TR_FEW, TR_MANY>(L, request(L, b));
+            base += s.tiles * chunks(s) * (int)L.kv.d;
+        }
+        if (tid == NT - 1) pre[B] = total;
+        __syncthreads();
+    }
+    // item `id`: its place in its request; false where no row of the tile sees a key of the chunk
+    __device__ inline bool item(const Launch& L, const int* pre, int id, Item& it, int& tr) const {
+        int at;
+        if (L.a.n_seq <= 64) {
+            it.b = __builtin_popcountll(__ballot(incl <= id));           // requests that end before it
+            it.rq.r0 = __builtin_amdgcn_readlane(mine.r0, it.b);
+            it.rq.r1 = __builtin_amdgcn_readlane(mine.r1, it.b);
+            it.rq.len = __builtin_amdgcn_readlane(mine.len, it.b);
+            at = id - (it.b ? __builtin_amdgcn_readlane(incl, it.b - 1) : 0);
+        } else {
+            it.b = __builtin_amdgcn_readfirstlane(m5_upper(pre, L.a.n_seq, id));
+            it.rq = request(L, it.b);
+            at = id - __builtin_amdgcn_readfirstlane(pre[it.b]);
+        }
+        const Share s = share_of<TR_FEW, TR_MANY>(L, it.rq);
+        const int nc = chunks(s), rest = L.kv.div(at);
+        it.kvh = at - rest * (int)L.kv.d;
+        const int up = nc == 1 ? rest : (int)((uint32_t)rest / (uint32_t)nc), chunk = rest - up * nc;
+        it.rho0 = (s.tiles - 1 - up) * s.tr;                 // the longest rows first
+        it.rho1 = min(it.rho0 + s.tr, s.rows);
+        tr = s.tr;
+        const int pos0 = it.rq.len - (it.rq.r1 - it.rq.r0);
+        const int lo = m5_key_lo(pos0 + L.group.div(it.rho0), L.a.window), hi = m5_key_hi(pos0 + L.group.div(it.rho1 - 1), it.rq.len);
+        int c0 = 0, c1 = 0;
+        if (nc > 1 && hi > lo) {
+            c0 = (int)((uint32_t)((lo - s.k0) >> 6) / (uint32_t)cu);
+            c1 = (int)((uint32_t)((hi - 1 - s.k0) >> 6) / (uint32_t)cu);
+        }
+        if (chunk < c0 || chunk > c1) return false;
+        it.n_parts = c1 - c0 + 1;
+        if (it.n_parts > 1) {
+            const int64_t size = (int64_t)slot_rows * (HD + 2);              // rows of o, then (m, l) of each
+            const int first_id = id - (chunk - c0) * (int)L.kv.d;            // (ids of a tile's chunks are n_kv_heads apart)
+            it.slot = L.slots + id * size;
+            it.first_slot = L.slots + first_id * size;
+            it.part_stride = (int64_t)L.kv.d * size;
+            it.ticket = L.tickets + first_id;
+        }
+        it.ka = chunk > c0 ? s.k0 + chunk * cu * 64 : lo;
+        it.kb = chunk < c1 ? s.k0 + (chunk + 1) * cu * 64 : hi;
+        return true;
+    }
+};
+
+// R: row blocks of the few-row tiles; MANY: requests of more rows get 128-row tiles.
+template <typename T, int HD, int R, bool MANY>
 struct Shape {
-    using F = Few<T, HD, R, NW>;
-    static constexpr int TR = 16 * R, TRM = MANY ? 128 : 0, SLOT_ROWS = MANY ? 128 : TR;
+    using F = Few<T, HD, R>;
+    static constexpr int TR = 16 * R, TRM = MANY ? 128 : 0;
     static constexpr int RING_B = MANY ? (F::LDS_B > 4 * 64 * HD * 2 ? F::LDS_B : 4 * 64 * HD * 2) : F::LDS_B;
     static int lds_bytes(int n_seq) { return RING_B + IDS_B + ML_B + odd_bytes(HD) + (n_seq + 1) * 4; }
 };
 
-template <typename T, int HD, int R, int NW, bool MANY>
-__global__ __launch_bounds__(NT, MANY ? 2 : 1) void paged_attn_kernel(Launch L) {
+template <typename T, int HD, int R, bool MANY>
+__global__ __launch_bounds__(NT, MANY || (HD == 128 && R < 4 && T::EPL == 8) || (HD == 64 && R < 4) ? 2 : 1) void paged_attn_kernel(Launch L) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    using S = Shape<T, HD, R, NW, MANY>;
+    using S = Shape<T, HD, R, MANY>;
     int* ids = reinterpret_cast<int*>(lds + S::RING_B);
     float* ml = reinterpret_cast<float*>(lds + S::RING_B + IDS_B);
     int* sh = reinterpret_cast<int*>(lds + S::RING_B + IDS_B + NWAVE * 64 * 2 * 4);
     unsigned char* odd = lds + S::RING_B + IDS_B + ML_B;
     int* pre = reinterpret_cast<int*>(odd + odd_bytes(HD));
-    int64_t* red = reinterpret_cast<int64_t*>(ml);
-    const M5PagedAttnArgs& p = L.a;
-    const int B = p.n_seq, tid = threadIdx.x;
-    const int64_t cap = (int64_t)p.table_width << L.shift;
-
-    // ---- items: how long a chunk of keys is, and every request's first item
-    const int per = (B + NT - 1) / NT, b0 = min(tid * per, B), b1 = min(b0 + per, B);
-    int64_t units = 0, tiles = 0;
-    for (int b = b0; b < b1; ++b) {
-        const Share s = share_of<S::TR, S::TRM>(L, m5_request(p.q_start[b], p.q_start[b + 1], p.seq_len[b], p.n_rows, cap));
-        units += (int64_t)s.tiles * ((s.keys + 63) >> 6);
-        tiles += s.tiles;
-    }
-    units = block_sum64(units, red) * p.n_kv_heads;
-    tiles = block_sum64(tiles, red) * p.n_kv_heads;
-    // items <= units / (C / 64) + tiles, and a split item needs a slot
-    int64_t C = INT_MAX;
-    if (L.n_slots > tiles) {
-        C = max((units + L.target - 1) / L.target, (units + (L.n_slots - tiles) - 1) / (L.n_slots - tiles));
-        C = min(max(C, (int64_t)4) * 64, (int64_t)INT_MAX);
-    }
-    auto items_of = [&](const Share& s) { return max((int)((s.keys + C - 1) / C), 1); };
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) {
-        const Share s = share_of<S::TR, S::TRM>(L, m5_request(p.q_start[b], p.q_start[b + 1], p.seq_len[b], p.n_rows, cap));
-        mine += s.tiles * items_of(s) * p.n_kv_heads;
-    }
-    int incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(incl, d);
-        if ((tid & 63) >= d) incl += o;
-    }
-    __syncthreads();
-    if ((tid & 63) == 63) sh[tid >> 6] = incl;
-    __syncthreads();
-    int base = incl - mine, total = 0;
-    for (int w = 0; w < NWAVE; ++w) {
-        if (w < tid >> 6) base += sh[w];
-        total += sh[w];
-    }
-    for (int b = b0; b < b1; ++b) {
-        pre[b] = base;
-        const Share s = share_of<S::TR, S::TRM>(L, m5_request(p.q_start[b], p.q_start[b + 1], p.seq_len[b], p.n_rows, cap));
-        base += s.tiles * items_of(s) * p.n_kv_heads;
-    }
-    if (tid == NT - 1) pre[B] = total;
-    __syncthreads();
-
-    for (int id = blockIdx.x; id < total; id += gridDim.x) {
+    Deal<S::TR, S::TRM, HD> deal;
+    deal.setup(L, pre, ml, sh);
+    for (int id = blockIdx.x; id < deal.total; id += gridDim.x) {
         Item it;
-        it.b = m5_upper(pre, B, id);
-        it.rq = m5_request(p.q_start[it.b], p.q_start[it.b + 1], p.seq_len[it.b], p.n_rows, cap);
-        const Share s = share_of<S::TR, S::TRM>(L, it.rq);
-        const int nc = items_of(s), at = id - pre[it.b];
-        it.kvh = at % p.n_kv_heads;
-        const int chunk = at / p.n_kv_heads % nc, tile = s.tiles - 1 - at / p.n_kv_heads / nc;      // the longest rows first
-        it.rows = s.rows;
-        it.rho0 = tile * s.tr;
-        it.rho1 = min(it.rho0 + s.tr, s.rows);
-        it.id = id;
-        const int pos0 = it.rq.len - (it.rq.r1 - it.rq.r0);
-        const int lo = m5_key_lo(pos0 + it.rho0 / L.group, p.window), hi = m5_key_hi(pos0 + (it.rho1 - 1) / L.group, it.rq.len);
-        const int c0 = hi > lo ? (int)((lo - s.k0) / C) : 0, c1 = hi > lo ? (int)((hi - 1 - s.k0) / C) : 0;
-        if (chunk < c0 || chunk > c1) continue;                  // no row of this tile sees a key of this chunk
-        it.n_parts = c1 - c0 + 1;
-        it.first_id = id - (chunk - c0) * p.n_kv_heads;
-        it.ka = (int)max((int64_t)lo, s.k0 + chunk * C);
-        it.kb = (int)min((int64_t)hi, s.k0 + (chunk + 1) * C);
+        int tr;
+        if (!deal.item(L, pre, id, it, tr)) continue;
         if constexpr (MANY) {
-            if (s.tr == 128) {
+            if (tr == 128) {
                 Many<T, HD>::run(L, it, lds, ids, odd);
-                if (it.n_parts > 1) join_parts<T, HD, 128>(L, it, sh);
+                if (it.n_parts > 1) join_parts<T, HD, 128>(L, it, lds, sh);
                 __syncthreads();
                 continue;
             }
         }
         S::F::run(L, it, lds, ids, ml, odd);
-        if (it.n_parts > 1) join_parts<T, HD, S::TR>(L, it, sh);
+        if (it.n_parts > 1) join_parts<T, HD, S::TR>(L, it, lds, sh);
         __syncthreads();
     }
 }
 
-constexpr int MAX_SLOTS = 1024;
+
 
 // The tiling for these shapes: rows of a few-row tile, or 0 for the kernel with 128-row tiles.
 int tiling(int dtype, const M5PagedAttnArgs& a) {
@@ -764,19 +915,26 @@ int tiling(int dtype, const M5PagedAttnArgs& a) {
     return rows <= 64 || dtype == M5_F32 ? 64 : 0;
 }
 
-template <typename T, int HD, int R, int NW, bool MANY>
+// partial results of `rows` rows that fit `bytes` (with a 4-byte ticket each; a multiple of 4, so that what follows the tickets is aligned)
+int slots_of(int64_t bytes, int rows, int hd) {
+    return (int)min((int64_t)MAX_SLOTS, min(bytes, MAX_SLOT_BYTES) / ((int64_t)rows * (hd + 2) * 4 + 4)) & ~3;
+}
+
+template <typename T, int HD, int R, bool MANY>
 int launch_as(Launch& L, int cus, hipStream_t s) {
-    using S = Shape<T, HD, R, NW, MANY>;
+    using S = Shape<T, HD, R, MANY>;
     const int lds = S::lds_bytes(L.a.n_seq);
-    if (hipFuncSetAttribute((const void*)paged_attn_kernel<T, HD, R, NW, MANY>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return M5_ERR_LAUNCH;
-    L.slot_floats = (int64_t)S::SLOT_ROWS * (HD + 2);
-    L.n_slots = L.a.workspace ? (int)min((int64_t)MAX_SLOTS, L.a.workspace_bytes / (L.slot_floats * 4 + 4)) & ~3 : 0;     // (the slots behind the tickets stay 16-byte aligned)
+    if (hipFuncSetAttribute((const void*)paged_attn_kernel<T, HD, R, MANY>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return M5_ERR_LAUNCH;
+    L.n_few = slots_of(L.a.workspace ? L.a.workspace_bytes : 0, S::TR, HD);
+    L.n_big = MANY ? (int)min((int64_t)L.n_few, min(L.a.workspace ? L.a.workspace_bytes - L.n_few * 4 : 0, MAX_SLOT_BYTES) / (128 * (HD + 2) * 4)) : L.n_few;
     L.tickets = (int*)L.a.workspace;
-    L.slots = (float*)((char*)L.a.workspace + (int64_t)L.n_slots * 4);
-    L.target = 2 * cus * min(160 * 1024 / lds, 2);
-    const int64_t tiles = ((int64_t)L.a.n_rows * L.group / S::TR + L.a.n_seq) * L.a.n_kv_heads;      // upper bound
-    const int64_t grid = L.n_slots ? max((int64_t)L.target, tiles) : tiles;
-    hipLaunchKernelGGL((paged_attn_kernel<T, HD, R, NW, MANY>), dim3((unsigned)min(grid, (int64_t)1 << 20)), dim3(NT), lds, s, L);
+    L.slots = (float*)((char*)L.a.workspace + (int64_t)L.n_few * 4);         // (n_few is a multiple of 4)
+    L.places = cus * min(160 * 1024 / lds, 2);
+    const int64_t tiles = ((int64_t)L.a.n_rows * L.group.d / S::TR + L.a.n_seq) * L.a.n_kv_heads;      // upper bound
+    // a workgroup for every item there can be; a workgroup takes several where that is too many
+    const int64_t chunks = (((int64_t)L.a.table_width << L.shift) + 64 * MIN_UNITS - 1) / (64 * MIN_UNITS);
+    const int64_t grid = L.n_few ? max(min((int64_t)4 * L.places, tiles * chunks), tiles) : tiles;
+    hipLaunchKernelGGL((paged_attn_kernel<T, HD, R, MANY>), dim3((unsigned)min(grid, (int64_t)1 << 20)), dim3(NT), lds, s, L);
     M5_CHECK_LAUNCH();
     return M5_OK;
 }
@@ -793,7 +951,7 @@ int check(int dtype, const M5PagedAttnArgs* a) {
         return M5_ERR_ARG;
     if (dtype != M5_F32 && dtype != M5_F16 && dtype != M5_BF16) return M5_ERR_UNSUPPORTED;
     if ((a->head_dim != 64 && a->head_dim != 128) || a->block_size > 1024 || a->n_seq > MAX_SEQ || ((int64_t)a->table_width << shift) > (1 << 30) ||
-        ((int64_t)a->n_blocks << shift) > INT_MAX || (int64_t)a->n_rows * a->n_heads > INT_MAX / 4)
+        ((int64_t)a->n_blocks << shift) > INT_MAX || (int64_t)a->n_rows * a->n_heads > (1 << 28) || (int64_t)a->n_seq * a->n_kv_heads > (1 << 28))
         return M5_ERR_UNSUPPORTED;
     const int epl = dtype == M5_F32 ? 4 : 8;
     if (!aligned(a->q, a->q_rs, a->q_hs, 0, epl) || !aligned(a->out, a->o_rs, a->o_hs, 0, epl) || !aligned(a->k_cache, a->k_bs, a->k_hs, a->k_ss, epl) ||
@@ -809,19 +967,20 @@ int launch(const M5PagedAttnArgs& a, int shift, hipStream_t s) {
     Launch L;
     L.a = a;
     L.shift = shift;
-    L.group = a.n_heads / a.n_kv_heads;
+    L.group.set(a.n_heads / a.n_kv_heads);
+    L.kv.set(a.n_kv_heads);
     L.sc2 = a.scale * 1.4426950408889634f;
     const int tr = tiling(T::id, a);
     if (a.head_dim == 64) {
         if constexpr (T::id != M5_F32)
-            if (tr == 0) return launch_as<T, 64, 2, 4, true>(L, cus, s);
-        return tr == 16 ? launch_as<T, 64, 1, 4, false>(L, cus, s) : tr == 32 ? launch_as<T, 64, 2, 4, false>(L, cus, s) : launch_as<T, 64, 4, 4, false>(L, cus, s);
+            if (tr == 0) return launch_as<T, 64, 2, true>(L, cus, s);
+        return tr == 16 ? launch_as<T, 64, 1, false>(L, cus, s) : tr == 32 ? launch_as<T, 64, 2, false>(L, cus, s) : launch_as<T, 64, 4, false>(L, cus, s);
     }
     if constexpr (T::id != M5_F32) {
-        if (tr == 0) return launch_as<T, 128, 2, 2, true>(L, cus, s);
-        if (tr == 64) return launch_as<T, 128, 4, 4, false>(L, cus, s);
+        if (tr == 0) return launch_as<T, 128, 2, true>(L, cus, s);
+        if (tr == 64) return launch_as<T, 128, 4, false>(L, cus, s);
     }
-    return tr == 16 ? launch_as<T, 128, 1, 4, false>(L, cus, s) : launch_as<T, 128, 2, 4, false>(L, cus, s);
+    return tr == 16 ? launch_as<T, 128, 1, false>(L, cus, s) : launch_as<T, 128, 2, false>(L, cus, s);
 }
 
 }  // namespace
@@ -831,7 +990,8 @@ extern "C" int m5_paged_attention_workspace(int dtype, const M5PagedAttnArgs* a,
     if (rc != M5_OK) return rc;
     if (!bytes) return M5_ERR_ARG;
     const int tr = tiling(dtype, *a);
-    *bytes = (int64_t)MAX_SLOTS * ((int64_t)(tr ? tr : 128) * (a->head_dim + 2) * 4 + 4);
+    const int rows = tr ? tr : 128;
+    *bytes = (int64_t)slots_of(MAX_SLOT_BYTES, rows, a->head_dim) * ((int64_t)rows * (a->head_dim + 2) * 4 + 4);
     return M5_OK;
 }
 
