@@ -25,6 +25,7 @@
 #include "common.h"
 #include "paged_index.h"
 #include <limits.h>
+#include <initializer_list>
 #include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) _Float16 h8_t;
@@ -64,6 +65,7 @@ struct Launch {
     int n_big, n_few;                            // partial results of the largest / of few-row tiles that the workspace holds (0: keys are not split)
     float* slots; int* tickets;
     float sc2;                                   // scale * log2(e)
+    uint32_t k_bs16, k_ss16, v_bs16, v_ss16;     // block and slot strides in 16-byte units
 };
 
 struct Item {
@@ -154,9 +156,20 @@ __device__ inline float infinite_part(bool up, bool down) { return (up ? INFINIT
 __device__ inline unsigned long long below(int n) { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1); }
 __device__ inline unsigned long long seen(unsigned long long there, int kb, int lo, int hi) { return there & below(hi - kb + 1) & ~below(lo - kb); }
 
-// block id of a key through the segment's ids in LDS, -1 outside [ka, kb)
-__device__ inline int key_block(const int* ids, int page0, int key, int ka, int kb, int shift) {
-    return key >= ka && key < kb ? ids[(key >> shift) - page0] : -1;
+// block id of a key through the segment's ids in LDS (ids: where page 0 would be), -1 outside [ka, kb)
+__device__ inline int key_block(const int* ids, int key, int ka, int kb, int shift) {
+    return key >= ka && key < kb ? ids[key >> shift] : -1;
+}
+// What the DMA reads for a key: the 16-byte chunk `ch` of its row; outside [ka, kb) the nearest key's, on a bad page block 0's (a
+// valid address: such keys are masked).  32 x 32 + 64-bit arithmetic in 16-byte units: with 64-bit strides the addresses of a tile cost
+// as much as its softmax (8 chunks of 2048 keys of 128 features: TODO against 743 TFLOP/s).
+struct RowAt { uint32_t id, off; };
+__device__ inline RowAt row_at(const int* ids, int key, int ka, int kb, int shift) {
+    const int k = min(max(key, ka), kb - 1);
+    return {(uint32_t)max(ids[k >> shift], 0), (uint32_t)k & ((1u << shift) - 1)};
+}
+__device__ inline const unsigned char* row_chunk(const unsigned char* base, RowAt r, uint32_t bs16, uint32_t ss16, uint32_t ch) {
+    return base + (((uint64_t)r.id * bs16 + (__umul24(r.off, ss16) + ch)) << 4);
 }
 
 // Partial results cross between workgroups (and XCDs, whose L2s do not share lines) as agent-scope accesses: written through to memory and
@@ -277,7 +290,6 @@ struct Few {
         uint32_t* down = up + HD;
         const unsigned char* Kg = (const unsigned char*)p.k_cache + (int64_t)it.kvh * p.k_hs * ES;
         const unsigned char* Vg = (const unsigned char*)p.v_cache + (int64_t)it.kvh * p.v_hs * ES;
-        const int off_mask = (1 << L.shift) - 1;
         const int step = NWAVE * KS;                                // keys of one round of the waves
         const int64_t seg = ((int64_t)(MAXP - 1) << L.shift) / step * step;
         const int k_first = it.ka & ~(KS - 1);
@@ -286,6 +298,7 @@ struct Few {
         for (int64_t s0 = k_first; s0 < it.kb; s0 += seg) {
             const int s1 = (int)min((int64_t)it.kb, s0 + seg);
             const int page0 = (int)s0 >> L.shift, np = ((s1 - 1) >> L.shift) - page0 + 1;
+            const int* id0 = ids - page0;
             __syncthreads();
             for (int i = tid; i < np; i += NT) ids[i] = m5_block(p.block_table[(int64_t)it.b * p.table_rs + page0 + i], p.n_blocks);
             __syncthreads();
@@ -294,16 +307,15 @@ struct Few {
 #pragma unroll
                 for (int j = 0; j < NI; ++j) {
                     const int row = j * RPI + lane / LPR, ch = lane % LPR;
-                    const int id = key_block(ids, page0, kb + row, it.ka, s1, L.shift);
-                    const int64_t blk = max(id, 0), off = id < 0 ? 0 : (kb + row) & off_mask;
-                    glds16(Kg + (blk * p.k_bs + off * p.k_ss) * ES + ((ch ^ kswz(row)) << 4), to + j * 1024);
-                    glds16(Vg + (blk * p.v_bs + off * p.v_ss) * ES + ((ch ^ vswz(row)) << 4), to + OP_B + j * 1024);
+                    const RowAt at = row_at(id0, kb + row, it.ka, s1, L.shift);
+                    glds16(row_chunk(Kg, at, L.k_bs16, L.k_ss16, ch ^ kswz(row)), to + j * 1024);
+                    glds16(row_chunk(Vg, at, L.v_bs16, L.v_ss16, ch ^ vswz(row)), to + OP_B + j * 1024);
                 }
             };
             auto block = [&](int kb, int stage) {
                 const unsigned char* ks = mine + stage * STAGE_B;
                 const unsigned char* vs = ks + OP_B;
-                const uint32_t there = (uint32_t)__ballot(key_block(ids, page0, kb + (lane & (KS - 1)), it.ka, s1, L.shift) >= 0) & (uint32_t)((1ull << KS) - 1);
+                const uint32_t there = (uint32_t)__ballot(key_block(id0, kb + (lane & (KS - 1)), it.ka, s1, L.shift) >= 0) & (uint32_t)((1ull << KS) - 1);
                 const bool whole = there == (uint32_t)((1ull << KS) - 1) && kb + KS - 1 <= pos_min && kb >= lo_max;
                 const bool odd = !whole && clean(mine + stage * STAGE_B + OP_B, there, up, down);
                 uint32_t vis[R];
@@ -515,13 +527,13 @@ struct Many {
         const int first_pos = pos0 + L.group.div(it.rho0), last_lo = m5_key_lo(pos0 + L.group.div(it.rho1 - 1), p.window);      // of all rows here
         const unsigned char* Kg = (const unsigned char*)p.k_cache + (int64_t)it.kvh * p.k_hs * 2;
         const unsigned char* Vg = (const unsigned char*)p.v_cache + (int64_t)it.kvh * p.v_hs * 2;
-        const int off_mask = (1 << L.shift) - 1;
         const int64_t seg = ((int64_t)(MAXP - 1) << L.shift) / KT * KT;
 
         vm_wait<0>();
         for (int64_t s0 = it.ka & ~(KT - 1); s0 < it.kb; s0 += seg) {
             const int s1 = (int)min((int64_t)it.kb, s0 + seg);
             const int page0 = (int)s0 >> L.shift, np = ((s1 - 1) >> L.shift) - page0 + 1;
+            const int* id0 = ids - page0;
             __syncthreads();
             for (int i = tid; i < np; i += NT) ids[i] = m5_block(p.block_table[(int64_t)it.b * p.table_rs + page0 + i], p.n_blocks);
             __syncthreads();
@@ -530,10 +542,9 @@ struct Many {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const int row = (wave * NJ + j) * RPI + lane / LPR, ch = lane % LPR;
-                    const int id = key_block(ids, page0, kb + row, it.ka, s1, L.shift);
-                    const int64_t blk = max(id, 0), off = id < 0 ? 0 : (kb + row) & off_mask;
-                    glds16(Kg + (blk * p.k_bs + off * p.k_ss) * 2 + ((ch ^ kswz(row)) << 4), to + j * 1024);
-                    glds16(Vg + (blk * p.v_bs + off * p.v_ss) * 2 + ((ch ^ vswz(row)) << 4), to + OP_B + j * 1024);
+                    const RowAt at = row_at(id0, kb + row, it.ka, s1, L.shift);
+                    glds16(row_chunk(Kg, at, L.k_bs16, L.k_ss16, ch ^ kswz(row)), to + j * 1024);
+                    glds16(row_chunk(Vg, at, L.v_bs16, L.v_ss16, ch ^ vswz(row)), to + OP_B + j * 1024);
                 }
             };
             auto tile = [&](int kb, int stage, unsigned long long there, bool odd) {
@@ -612,7 +623,7 @@ struct Many {
                 vm_wait<0>();
                 __syncthreads();                                 // the tile is there for all waves, and all are done with the other stage
                 if (kb + KT < s1) fetch(kb + KT, stage ^ 1);
-                const unsigned long long there = __ballot(key_block(ids, page0, kb + lane, it.ka, s1, L.shift) >= 0);
+                const unsigned long long there = __ballot(key_block(id0, kb + lane, it.ka, s1, L.shift) >= 0);
                 const bool odd = !(there == ~0ull && kb + KT - 1 <= first_pos && kb >= last_lo) && clean(lds + stage * STAGE_B + OP_B, there, up, down);
                 if (w0 < w1 && kb <= pos_max && kb + KT > lo_min) tile(kb, stage, there, odd);
             }
@@ -774,8 +785,9 @@ struct Deal {
         cu = INT_MAX >> 7;
         if (tiles < slots) {
             const float room = min(4.f * tiles <= P ? P - tiles : (tiles <= 2.f * P ? 4.f * P - tiles : 0.5f * P), slots - tiles);
-            const float len = max(units * 1.0001f / room + 1.f, units / (128.f * max(tiles, 1.f)));      // at most about 128 parts to a tile
-            cu = (int)min(max(len, (float)MIN_UNITS), (float)(INT_MAX >> 7));
+            // a tile of u units in n parts takes about a u / n + b n (the join): no shorter than sqrt(b u / a)
+            const float least = max((float)MIN_UNITS, (MANY && slot_rows == TR_MANY ? 2.2f : 1.f) * sqrtf(units / max(tiles, 1.f)));
+            cu = (int)min(max(units * 1.0001f / room + 1.f, least), (float)(INT_MAX >> 7));
         }
     }
     __device__ inline M5Request request(const Launch& L, int b) const {
@@ -911,8 +923,8 @@ __global__ __launch_bounds__(NT, MANY || (HD == 128 && R < 4 && T::EPL == 8) || 
 int tiling(int dtype, const M5PagedAttnArgs& a) {
     const int64_t rows = (int64_t)min(max(a.max_new, 1), max(a.n_rows, 1)) * (a.n_heads / a.n_kv_heads);
     if (rows <= 16) return 16;
-    if (rows <= 32 || (dtype == M5_F32 && a.head_dim == 128)) return 32;             // (64 fp32 rows of 128 features: too many registers)
-    return rows <= 64 || dtype == M5_F32 ? 64 : 0;
+    if (rows <= 32 || dtype == M5_F32) return 32;            // (64 fp32 rows need the registers of two waves: 2 x 1000 rows 570 us against 375)
+    return rows <= 64 ? 64 : 0;
 }
 
 // partial results of `rows` rows that fit `bytes` (with a 4-byte ticket each; a multiple of 4, so that what follows the tickets is aligned)
@@ -957,6 +969,11 @@ int check(int dtype, const M5PagedAttnArgs* a) {
     if (!aligned(a->q, a->q_rs, a->q_hs, 0, epl) || !aligned(a->out, a->o_rs, a->o_hs, 0, epl) || !aligned(a->k_cache, a->k_bs, a->k_hs, a->k_ss, epl) ||
         !aligned(a->v_cache, a->v_bs, a->v_hs, a->v_ss, epl) || ((uintptr_t)a->workspace & 15))
         return M5_ERR_UNSUPPORTED;
+    // strides of blocks below 64 GB, of slots below 64 MB (row_chunk)
+    for (int64_t bs : {a->k_bs, a->v_bs})
+        if (bs < 0 || bs / epl > UINT32_MAX) return M5_ERR_UNSUPPORTED;
+    for (int64_t ss : {a->k_ss, a->v_ss})
+        if (ss < 0 || ss / epl > (1 << 22)) return M5_ERR_UNSUPPORTED;
     return M5_OK;
 }
 
@@ -970,11 +987,18 @@ int launch(const M5PagedAttnArgs& a, int shift, hipStream_t s) {
     L.group.set(a.n_heads / a.n_kv_heads);
     L.kv.set(a.n_kv_heads);
     L.sc2 = a.scale * 1.4426950408889634f;
+    constexpr int E = T::EPL;
+    L.k_bs16 = (uint32_t)(a.k_bs / E);
+    L.k_ss16 = (uint32_t)(a.k_ss / E);
+    L.v_bs16 = (uint32_t)(a.v_bs / E);
+    L.v_ss16 = (uint32_t)(a.v_ss / E);
     const int tr = tiling(T::id, a);
     if (a.head_dim == 64) {
-        if constexpr (T::id != M5_F32)
+        if constexpr (T::id != M5_F32) {
             if (tr == 0) return launch_as<T, 64, 2, true>(L, cus, s);
-        return tr == 16 ? launch_as<T, 64, 1, false>(L, cus, s) : tr == 32 ? launch_as<T, 64, 2, false>(L, cus, s) : launch_as<T, 64, 4, false>(L, cus, s);
+            if (tr == 64) return launch_as<T, 64, 4, false>(L, cus, s);
+        }
+        return tr == 16 ? launch_as<T, 64, 1, false>(L, cus, s) : launch_as<T, 64, 2, false>(L, cus, s);
     }
     if constexpr (T::id != M5_F32) {
         if (tr == 0) return launch_as<T, 128, 2, true>(L, cus, s);
