@@ -36,6 +36,7 @@ typedef __attribute__((ext_vector_type(4))) short s4_t;
 
 namespace {
 
+constexpr int SCHED_MFMA = 0x8, SCHED_DS = 0x100;        // sched_group_barrier: matrix instructions, LDS reads
 constexpr int NWAVE = 4, NT = NWAVE * 64;
 constexpr int MAXP = 1024;                       // block ids of one key segment held in LDS
 constexpr int MAX_SLOTS = 4096;                  // partial results of a call, and their bytes
@@ -110,6 +111,20 @@ __device__ inline void glds16(const unsigned char* gsrc, uint32_t lds_base) {
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(gsrc), "s"(lds_base) : "memory");
 }
+// the same from a wave-uniform base and a 32-bit byte offset per lane
+__device__ inline void glds16(const unsigned char* base, uint32_t off, uint32_t lds_base) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(lds_base), "s"(base) : "memory");
+}
+__device__ inline const unsigned char* uniform(const unsigned char* p) {
+    const uint64_t v = (uint64_t)p;
+    return (const unsigned char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
+}
+__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }      // (a value that the compiler does not see is uniform)
+// The loads of v are waited for HERE: left to their first use inside the key loop, the compiler would wait there in every round, and with
+// them for the DMA in flight.
+__device__ inline void arrived(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
 template <int N>
 __device__ inline void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 __device__ inline void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -233,7 +248,8 @@ struct Few {
 
     // V of a stage that not all rows see whole: keys that are not there become zeros, non-finite values are noted and taken out (true).
     __device__ static bool clean(unsigned char* vs, uint32_t there, uint32_t* up, uint32_t* down) {
-        const int lane = threadIdx.x & 63;
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));                           // (addresses of this rare path are not to be kept in registers through the key loop)
         uint32_t any = 0;
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
@@ -274,7 +290,7 @@ struct Few {
 #pragma unroll
             for (int t = 0; t < NF; ++t) qf[rb][t] = *reinterpret_cast<const uint4*>(q + (4 * t + g) * T::EPL);
         }
-        const int pos_min = pos0 + L.group.div(it.rho0), pos_max = pos0 + L.group.div(it.rho1 - 1);
+        const int pos_min = uniform(pos0 + L.group.div(it.rho0)), pos_max = uniform(pos0 + L.group.div(it.rho1 - 1));
         const int lo_max = m5_key_lo(pos_max, p.window);         // the last row's first key
         f4_t o[R][ND];
         Soft sm[R];
@@ -294,6 +310,10 @@ struct Few {
         const int64_t seg = ((int64_t)(MAXP - 1) << L.shift) / step * step;
         const int k_first = it.ka & ~(KS - 1);
 
+#pragma unroll
+        for (int rb = 0; rb < R; ++rb)
+#pragma unroll
+            for (int t = 0; t < NF; ++t) arrived(qf[rb][t]);
         vm_wait<0>();                                            // nothing of an earlier item is in flight
         for (int64_t s0 = k_first; s0 < it.kb; s0 += seg) {
             const int s1 = (int)min((int64_t)it.kb, s0 + seg);
@@ -393,17 +413,20 @@ struct Few {
                     for (int rb = 0; rb < R; ++rb)
                         if (R == 1 || rb < nrb) o[rb][d] = mma16(v, pf[rb], o[rb][d], T());
                 }
-                if (odd)
+                if (odd) {
+                    int at = 4 * g;
+                    asm volatile("" : "+v"(at));                 // (computed here: the compiler would keep an address per feature in registers)
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            asm volatile("" ::: "memory");       // (one feature's notes at a time: read ahead they would cost registers)
-                            const uint32_t u = up[16 * d + 4 * g + r], n = down[16 * d + 4 * g + r];
+                            asm volatile("" ::: "memory");       // (one feature's notes at a time)
+                            const uint32_t u = up[at + 16 * d + r], n = down[at + 16 * d + r];
 #pragma unroll
                             for (int rb = 0; rb < R; ++rb)
                                 if (R == 1 || rb < nrb) o[rb][d][r] += infinite_part(u & vis[rb], n & vis[rb]);
                         }
+                }
             };
             int kb = (int)s0 + wave * KS, stage = 0;
             if (kb < s1) fetch(kb, 0);
@@ -474,7 +497,8 @@ struct Many {
 
     // As Few::clean, by the whole workgroup (every wave calls it; the barriers inside also order it before the waves' reads).
     __device__ static bool clean(unsigned char* vs, unsigned long long there, unsigned long long* up, unsigned long long* down) {
-        const int tid = threadIdx.x;
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));                            // (as there)
         constexpr int N = OP_B / (NT * 16);
         uint32_t any = 0;
 #pragma unroll
@@ -507,7 +531,7 @@ struct Many {
         const int w0 = it.rho0 + wave * 32, w1 = min(w0 + 32, it.rho1);      // this wave's rows (none: it only fetches)
         const int pos0 = it.rq.len - (it.rq.r1 - it.rq.r0);
         const int rho = min(w0 + c, it.rho1 - 1), tok = L.group.div(rho), qpos = pos0 + tok;
-        const int pos_min = pos0 + L.group.div(w0), pos_max = pos0 + L.group.div(max(w1 - 1, 0));
+        const int pos_min = uniform(pos0 + L.group.div(w0)), pos_max = uniform(pos0 + L.group.div(max(w1 - 1, 0)));
         const int lo_min = m5_key_lo(pos_min, p.window), lo_max = m5_key_lo(pos_max, p.window), lo = m5_key_lo(qpos, p.window);
         uint4 qf[NF];
         {
@@ -520,31 +544,57 @@ struct Many {
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-        Soft sm = {-INFINITY, 0.f};
+        float m = -INFINITY, use = 0.f, l = 0.f;
+        const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);      // bf16
         const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
         unsigned long long* up = reinterpret_cast<unsigned long long*>(odd_lds);
         unsigned long long* down = up + HD;
-        const int first_pos = pos0 + L.group.div(it.rho0), last_lo = m5_key_lo(pos0 + L.group.div(it.rho1 - 1), p.window);      // of all rows here
+        const int first_pos = uniform(pos0 + L.group.div(it.rho0)), last_lo = m5_key_lo(uniform(pos0 + L.group.div(it.rho1 - 1)), p.window);      // of all rows here
         const unsigned char* Kg = (const unsigned char*)p.k_cache + (int64_t)it.kvh * p.k_hs * 2;
         const unsigned char* Vg = (const unsigned char*)p.v_cache + (int64_t)it.kvh * p.v_hs * 2;
-        const int64_t seg = ((int64_t)(MAXP - 1) << L.shift) / KT * KT;
+        const int seg = (int)min(((int64_t)(MAXP - 1) << L.shift) / KT * KT, (int64_t)1 << 30);
+        const uint32_t mask = (1u << L.shift) - 1;
+        // A DMA instruction reads RPI consecutive rows; pages of at least as many hold them together, so the page is wave-uniform and only
+        // the offset inside it is the lane's (constant): no vector address arithmetic in the loop (c128: TODO).
+        const bool one_page = mask + 1 >= RPI;
+        uint32_t k_off[NJ], v_off[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int row = (wave * NJ + j) * RPI + lane / LPR, ch = lane % LPR;
+            k_off[j] = (lane / LPR * L.k_ss16 + (ch ^ kswz(row))) << 4;
+            v_off[j] = (lane / LPR * L.v_ss16 + (ch ^ vswz(row))) << 4;
+        }
 
+#pragma unroll
+        for (int t = 0; t < NF; ++t) arrived(qf[t]);
         vm_wait<0>();
-        for (int64_t s0 = it.ka & ~(KT - 1); s0 < it.kb; s0 += seg) {
-            const int s1 = (int)min((int64_t)it.kb, s0 + seg);
-            const int page0 = (int)s0 >> L.shift, np = ((s1 - 1) >> L.shift) - page0 + 1;
+        for (int s0 = it.ka & ~(KT - 1); s0 < it.kb; s0 += seg) {
+            const int s1 = uniform(min(it.kb, s0 + seg));
+            const int page0 = s0 >> L.shift, np = ((s1 - 1) >> L.shift) - page0 + 1;
             const int* id0 = ids - page0;
             __syncthreads();
-            for (int i = tid; i < np; i += NT) ids[i] = m5_block(p.block_table[(int64_t)it.b * p.table_rs + page0 + i], p.n_blocks);
-            __syncthreads();
-            auto fetch = [&](int kb, int stage) {
+            int bad = 0;
+            for (int i = tid; i < np; i += NT) {
+                ids[i] = m5_block(p.block_table[(int64_t)it.b * p.table_rs + page0 + i], p.n_blocks);
+                bad |= ids[i] < 0;
+            }
+            const bool some_bad = __syncthreads_or(bad);
+            // lane j: the block of this wave's j-th instruction of the tile at kb
+            auto blocks_of = [&](int kb) { return row_at(id0, kb + (wave * NJ + min(lane, NJ - 1)) * RPI, it.ka, s1, L.shift).id; };
+            auto fetch = [&](int kb, int stage, uint32_t blocks) {
                 const uint32_t to = ring + stage * STAGE_B + wave * NJ * 1024;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    const int row = (wave * NJ + j) * RPI + lane / LPR, ch = lane % LPR;
-                    const RowAt at = row_at(id0, kb + row, it.ka, s1, L.shift);
-                    glds16(row_chunk(Kg, at, L.k_bs16, L.k_ss16, ch ^ kswz(row)), to + j * 1024);
-                    glds16(row_chunk(Vg, at, L.v_bs16, L.v_ss16, ch ^ vswz(row)), to + OP_B + j * 1024);
+                    if (one_page) {
+                        const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)blocks, j), off = (uint32_t)(kb + (wave * NJ + j) * RPI) & mask;
+                        glds16(uniform(Kg + (((uint64_t)id * L.k_bs16 + off * L.k_ss16) << 4)), k_off[j], to + j * 1024);
+                        glds16(uniform(Vg + (((uint64_t)id * L.v_bs16 + off * L.v_ss16) << 4)), v_off[j], to + OP_B + j * 1024);
+                    } else {
+                        const int row = (wave * NJ + j) * RPI + lane / LPR, ch = lane % LPR;
+                        const RowAt at = row_at(id0, kb + row, it.ka, s1, L.shift);
+                        glds16(row_chunk(Kg, at, L.k_bs16, L.k_ss16, ch ^ kswz(row)), to + j * 1024);
+                        glds16(row_chunk(Vg, at, L.v_bs16, L.v_ss16, ch ^ vswz(row)), to + OP_B + j * 1024);
+                    }
                 }
             };
             auto tile = [&](int kb, int stage, unsigned long long there, bool odd) {
@@ -553,15 +603,30 @@ struct Many {
                 const bool whole = there == ~0ull && kb + KT - 1 <= pos_min && kb >= lo_max;
                 unsigned long long vis = 0;
                 f16_t s[2];
+                uint4 kf[2][NF];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int t = 0; t < NF; ++t) {
+                        const int row = 32 * h + c;
+                        kf[h][t] = *reinterpret_cast<const uint4*>(ks + row * RB + (((2 * t + hh) ^ kswz(row)) << 4));
+                    }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[h][r] = 0.f;
-                    const int row = 32 * h + c;
 #pragma unroll
-                    for (int t = 0; t < NF; ++t)
-                        s[h] = mma32(*reinterpret_cast<const uint4*>(ks + row * RB + (((2 * t + hh) ^ kswz(row)) << 4)), qf[t], s[h], T());
+                    for (int t = 0; t < NF; ++t) s[h] = mma32(kf[h][t], qf[t], s[h], T());
                 }
+                // one key block's fragments ahead of the products (left to itself the compiler reads each fragment into the same registers and
+                // waits for it: an LDS round trip per product)
+                __builtin_amdgcn_sched_group_barrier(SCHED_DS, NF, 0);
+#pragma unroll
+                for (int t = 0; t < NF; ++t) {
+                    __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(SCHED_DS, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, NF, 0);
                 if (!whole) {
                     vis = seen(there, kb, lo, qpos);
 #pragma unroll
@@ -575,65 +640,90 @@ struct Many {
 #pragma unroll
                 for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, s[0][r]), s[1][r]);
                 mx = fmaxf(mx, lane_xor32(mx)) * L.sc2;
-                float use, sum = 0.f;
-                const float alpha = sm.step(mx, use);
+                // p = exp2(s - m) with an m that is raised only when a score passes it by more than 8: p stays below 2^8, which the operand
+                // types hold with the same relative error, and most tiles spare the rescaling of o (64 or 32 products per lane)
+                if (__any(mx > m + 8.f)) {
+                    const float mn = fmaxf(m, mx);
+                    use = mn == -INFINITY ? 0.f : mn;
+                    const float alpha = __builtin_amdgcn_exp2f(m - use);
+                    m = mn;
+                    l *= alpha;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) o[d] *= alpha;
+                }
                 uint4 pf[2][2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
+                    for (int k = 0; k < 2; ++k) {
                         st e[8];
+                        float x[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][8 * m + j], L.sc2, -use));
-                            sum += x;
-                            e[j] = T::from_f32(x);
+                            x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][8 * k + j], L.sc2, -use));
+                            e[j] = T::from_f32(x[j]);
                         }
-                        pf[h][m] = *reinterpret_cast<const uint4*>(e);
+                        pf[h][k] = *reinterpret_cast<const uint4*>(e);
+                        // the denominator in fp32: of the rounded pairs (bf16: one instruction a pair), of the values (fp16, whose small
+                        // p the pair instruction might take for zero)
+                        if constexpr (T::id == M5_BF16) l = dot8<T>(pf[h][k], ones, l);
+                        else
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) l += x[j];
                     }
-                sm.l = sm.l * alpha + sum;
-                if (!__all(alpha == 1.0f))
+                uint4 vf[4][ND];
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) o[d] *= alpha;
+                for (int k = 0; k < 4; ++k)                      // 16 keys at a time
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int d = 0; d < ND; ++d) {
+                        const int row = 16 * k + 4 * hh + ((lane & 15) >> 2), ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+                        const uint2 v0 = tr_read(vs + row * RB + ((ch ^ vswz(row)) << 4) + (lane & 1) * 8);
+                        const uint2 v1 = tr_read(vs + (row + 8) * RB + ((ch ^ vswz(row + 8)) << 4) + (lane & 1) * 8);
+                        vf[k][d] = make_uint4(v0.x, v0.y, v1.x, v1.y);
+                    }
 #pragma unroll
-                    for (int m = 0; m < 2; ++m)
+                for (int k = 0; k < 4; ++k)
 #pragma unroll
-                        for (int d = 0; d < ND; ++d) {
-                            const int row = 32 * h + 16 * m + 4 * hh + ((lane & 15) >> 2), ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-                            const uint2 v0 = tr_read(vs + row * RB + ((ch ^ vswz(row)) << 4) + (lane & 1) * 8);
-                            const uint2 v1 = tr_read(vs + (row + 8) * RB + ((ch ^ vswz(row + 8)) << 4) + (lane & 1) * 8);
-                            const uint4 v = make_uint4(v0.x, v0.y, v1.x, v1.y);
-                            o[d] = mma32(v, pf[h][m], o[d], T());
-                        }
-                if (odd)
+                    for (int d = 0; d < ND; ++d) o[d] = mma32(vf[k][d], pf[k >> 1][k & 1], o[d], T());
+                __builtin_amdgcn_sched_group_barrier(SCHED_DS, 2 * ND, 1);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {                    // (as above, 16 keys ahead)
+                    __builtin_amdgcn_sched_group_barrier(SCHED_DS, 2 * ND, 1);
+                    __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, ND, 1);
+                }
+                __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, ND, 1);
+                if (odd) {
+                    int at = 4 * hh;
+                    asm volatile("" : "+v"(at));                 // (computed here: the compiler would keep an address per feature in registers)
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            const int at = 32 * d + 8 * (r >> 2) + 4 * hh + (r & 3);
-                            asm volatile("" ::: "memory");       // (one feature's notes at a time: read ahead they would cost registers)
-                            o[d][r] += infinite_part(up[at] & vis, down[at] & vis);
+                            asm volatile("" ::: "memory");       // (one feature's notes at a time)
+                            o[d][r] += infinite_part(up[at + 32 * d + 8 * (r >> 2) + (r & 3)] & vis, down[at + 32 * d + 8 * (r >> 2) + (r & 3)] & vis);
                         }
+                }
             };
             int stage = 0;
-            fetch((int)s0, 0);
-            for (int kb = (int)s0; kb < s1; kb += KT, stage ^= 1) {
+            fetch(s0, 0, blocks_of(s0));
+            uint32_t next = blocks_of(s0 + KT);
+            for (int kb = s0; kb < s1; kb += KT, stage ^= 1) {
                 vm_wait<0>();
                 __syncthreads();                                 // the tile is there for all waves, and all are done with the other stage
-                if (kb + KT < s1) fetch(kb + KT, stage ^ 1);
-                const unsigned long long there = __ballot(key_block(id0, kb + lane, it.ka, s1, L.shift) >= 0);
+                if (kb + KT < s1) fetch(kb + KT, stage ^ 1, next);
+                next = blocks_of(kb + 2 * KT);
+                unsigned long long there = seen(~0ull, kb, it.ka, s1 - 1);
+                if (some_bad) there = __ballot(key_block(id0, kb + lane, it.ka, s1, L.shift) >= 0);
                 const bool odd = !(there == ~0ull && kb + KT - 1 <= first_pos && kb >= last_lo) && clean(lds + stage * STAGE_B + OP_B, there, up, down);
                 if (w0 < w1 && kb <= pos_max && kb + KT > lo_min) tile(kb, stage, there, odd);
             }
         }
         if (w0 >= w1) return;
-        float l = sm.l + lane_xor32(sm.l);
+        l += lane_xor32(l);
         if (w0 + c >= w1) return;
         const int row = wave * 32 + c;
         float* slot = it.n_parts > 1 ? it.slot : nullptr;
-        if (slot && hh == 0) put_part(slot + 128 * HD + 2 * row, sm.m, l);
+        if (slot && hh == 0) put_part(slot + 128 * HD + 2 * row, m, l);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -643,7 +733,7 @@ struct Many {
                 if (slot) {
                     put_part(slot + row * HD + at, v[0], v[1]);
                     put_part(slot + row * HD + at + 2, v[2], v[3]);
-                } else put_row<T, HD>(L, it, row, at, v, sm.m, l);
+                } else put_row<T, HD>(L, it, row, at, v, m, l);
             }
     }
 };
@@ -875,6 +965,16 @@ struct Deal {
         }
         it.ka = chunk > c0 ? s.k0 + chunk * cu * 64 : lo;
         it.kb = chunk < c1 ? s.k0 + (chunk + 1) * cu * 64 : hi;
+        it.rho0 = uniform(it.rho0);
+        it.rho1 = uniform(it.rho1);
+        it.kvh = uniform(it.kvh);
+        it.ka = uniform(it.ka);
+        it.kb = uniform(it.kb);
+        it.n_parts = uniform(it.n_parts);
+        it.rq.r0 = uniform(it.rq.r0);
+        it.rq.r1 = uniform(it.rq.r1);
+        it.rq.len = uniform(it.rq.len);
+        tr = uniform(tr);
         return true;
     }
 };
