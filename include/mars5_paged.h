@@ -27,7 +27,7 @@
  *   state[M5_PST_STATUS] 0; > 0: that many blocks short; < 0: -1 - b = request b is not valid (a negative length, keep > held, more
  *                       positions than its table row holds), b = n_seq: more rows than n_rows, n_seq + 1: more blocks given back
  *                       than n_blocks.  Not 0 = nothing is taken or changed and the step has no rows: q_start 0, maps -1.
- * state: M5_PST_WORDS int32, zero-filled once, [M5_PST_FREE] set; words from 3 on are the library's.  n_seq <= 8192. */
+ * state: M5_PST_WORDS int32, zero-filled once, [M5_PST_FREE] set; words from 3 on are the library's.  n_seq <= 4096. */
 #define M5_PST_FREE 0
 #define M5_PST_STATUS 1
 #define M5_PST_ROWS 2

@@ -7,123 +7,163 @@
 namespace {
 
 // ---------------------------------------------------------------------------------------------------------- m5_paged_plan
-// Every workgroup scans the requests itself (three prefix sums into LDS: rows, blocks taken, blocks given back), so the rows and
-// blocks can be dealt to many workgroups without a second launch.  Nothing that any workgroup reads is written before the end:
-// table entries written lie behind the pages a growing request holds, those read as "given back" behind the pages a shrinking one
+// Every workgroup scans the requests itself (prefix sums of rows, blocks taken and blocks given back into LDS), so the rows and blocks can
+// be dealt to many workgroups without a second launch.  Nothing that any workgroup reads is written before the end: table
+// entries written lie behind the pages a growing request holds, those read as "given back" behind the pages a shrinking one
 // keeps, free-list entries written lie at or above n_free and those read below.  seq_len and the state words are written by the
 // workgroup that finishes last (ticket word of the state; it leaves the ticket at 0).
-constexpr int PLAN_NT = 1024;
-constexpr int PLAN_MAX_SEQ = 8192;
+// Latency bound: one memory round trip for the lengths, ~30 cross-lane adds, a search of log2(n_seq) LDS reads per row (four rows of a
+// thread at once) and one load per row.  4.3 us a call at 48 requests (graph replay), a launch's own time 2.7.
+constexpr int PLAN_MAX_SEQ = 4096;
 
-__device__ inline int64_t wave_scan(int64_t v) {             // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t o = __shfl_up((long long)v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
+template <int CTRL, int ROWS>
+__device__ inline int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ inline int wave_scan(int v) {                     // inclusive: row shifts, then the rows' last lanes broadcast
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    return dpp_add<0x143, 0xc>(v);
 }
 
-__global__ __launch_bounds__(PLAN_NT) void paged_plan_kernel(M5PagedPlanArgs p, int shift) {
-    extern __shared__ int pre[];                             // [3][n_seq + 1]
-    __shared__ int64_t wsum[3][PLAN_NT / 64];
+template <int NT>
+__global__ __launch_bounds__(NT) void paged_plan_kernel(M5PagedPlanArgs p, int shift) {
+    extern __shared__ int lds[];                             // [5][n_seq + 1]
+    __shared__ int wsum[NT / 64][4];
     __shared__ int first_bad, last;
     const int B = p.n_seq, tid = threadIdx.x, wave = tid >> 6;
-    int* row_pre = pre;
-    int* take_pre = pre + (B + 1);
-    int* give_pre = pre + 2 * (B + 1);
+    int* row_pre = lds;
+    int* take_pre = lds + (B + 1);
+    int* give_pre = lds + 2 * (B + 1);
+    int* keep = lds + 3 * (B + 1);
+    int* have = lds + 4 * (B + 1);                           // pages before the step
     if (tid == 0) first_bad = INT_MAX;
     const int n_free = m5_clampi(p.state[M5_PST_FREE], 0, p.n_blocks);
     __syncthreads();
 
-    const int per = (B + PLAN_NT - 1) / PLAN_NT;             // consecutive requests per thread
+    const int per = (B + NT - 1) / NT;                       // consecutive requests per thread
     const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
-    int64_t rows = 0, take = 0, give = 0;
+    int64_t rows = 0;
+    int take = 0, give = 0;
     for (int b = b0; b < b1; ++b) {
-        int have, need;
-        const int add = p.new_len[b];
-        if (!m5_plan_request(p.seq_len[b], p.keep_len[b], add, p.table_width, shift, have, need)) { atomicMin(&first_bad, b); continue; }
-        rows += add;
-        take += max(need - have, 0);
-        give += max(have - need, 0);
+        int h, need;
+        const int k = p.keep_len[b], add = p.new_len[b];
+        const bool ok = m5_plan_request(p.seq_len[b], k, add, p.table_width, shift, h, need);
+        if (!ok) atomicMin(&first_bad, b);
+        keep[b] = k;
+        have[b] = h;
+        row_pre[b] = ok ? add : 0;                           // (what it adds, for now)
+        take_pre[b] = need - h;
+        rows += ok ? add : 0;
+        take += max(need - h, 0);
+        give += max(h - need, 0);
     }
-    const int64_t ri = wave_scan(rows), ti = wave_scan(take), gi = wave_scan(give);
-    if ((tid & 63) == 63) { wsum[0][wave] = ri; wsum[1][wave] = ti; wsum[2][wave] = gi; }
+    // rows may pass 31 bits before they are found to be too many: scanned in two pieces of 20 and 12 bits
+    const int lo = wave_scan((int)(rows & 0xfffff)), hi = wave_scan((int)(rows >> 20)), ti = wave_scan(take), gi = wave_scan(give);
+    if ((tid & 63) == 63) { wsum[wave][0] = lo; wsum[wave][1] = hi; wsum[wave][2] = ti; wsum[wave][3] = gi; }
     __syncthreads();
-    int64_t rb = 0, tb = 0, gb = 0, n_rows = 0, n_take = 0, n_give = 0;
-    for (int w = 0; w < PLAN_NT / 64; ++w) {
+    int64_t rb = 0, n_rows = 0;
+    int tb = 0, gb = 0, n_take = 0, n_give = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
         if (w == wave) { rb = n_rows; tb = n_take; gb = n_give; }
-        n_rows += wsum[0][w];
-        n_take += wsum[1][w];
-        n_give += wsum[2][w];
+        n_rows += wsum[w][0] + ((int64_t)wsum[w][1] << 20);
+        n_take += wsum[w][2];
+        n_give += wsum[w][3];
     }
     int status = 0;
     if (first_bad != INT_MAX) status = -1 - first_bad;
     else if (n_rows > (p.slot_map ? p.n_rows : INT_MAX)) status = -1 - B;
-    else if (n_free + n_give - n_take > p.n_blocks) status = -2 - B;
-    else if (n_take > n_free + n_give) status = (int)(n_take - n_free - n_give);
+    else if ((int64_t)n_free + n_give - n_take > p.n_blocks) status = -2 - B;
+    else if (n_take > n_free + n_give) status = n_take - n_free - n_give;
     const bool ok = status == 0;                             // uniform over the grid
-    rb = ok ? rb + ri - rows : 0;
+    int rp = ok ? (int)(rb + lo + ((int64_t)hi << 20) - rows) : 0;
     tb = ok ? tb + ti - take : 0;
     gb = ok ? gb + gi - give : 0;
     for (int b = b0; b < b1; ++b) {                          // exclusive prefixes
-        row_pre[b] = (int)rb; take_pre[b] = (int)tb; give_pre[b] = (int)gb;
-        int have, need;
-        const int add = p.new_len[b];
-        m5_plan_request(p.seq_len[b], p.keep_len[b], add, p.table_width, shift, have, need);
-        if (ok) { rb += add; tb += max(need - have, 0); gb += max(have - need, 0); }
+        const int add = row_pre[b], d = take_pre[b];
+        row_pre[b] = rp; take_pre[b] = tb; give_pre[b] = gb;
+        if (ok) { rp += add; tb += max(d, 0); gb += max(-d, 0); }
     }
-    if (tid == PLAN_NT - 1) { row_pre[B] = ok ? (int)n_rows : 0; take_pre[B] = ok ? (int)n_take : 0; give_pre[B] = ok ? (int)n_give : 0; }
+    const int taken = ok ? n_take : 0, given = ok ? n_give : 0, described = ok ? (int)n_rows : 0;
+    if (tid == NT - 1) { row_pre[B] = described; take_pre[B] = taken; give_pre[B] = given; }
     __syncthreads();
 
-    const int taken = ok ? (int)n_take : 0, given = ok ? (int)n_give : 0, described = ok ? (int)n_rows : 0;
     auto returned = [&](int i) {                             // id of returned page i
-        const int b = m5_upper(give_pre, B, i);
-        const int need = m5_pages(p.keep_len[b] + p.new_len[b], shift);
+        const int b = m5_upper(give_pre, B, i), need = have[b] - (give_pre[b + 1] - give_pre[b]);
         return p.block_table[(int64_t)b * p.table_rs + need + (i - give_pre[b])];
     };
     auto allocation = [&](int a) {                           // id of allocation a
         const int src = m5_plan_source(a, given, n_free);
         return src >= 0 ? p.free_blocks[src] : returned(-1 - src);
     };
-    const int gt = blockIdx.x * PLAN_NT + tid, gn = gridDim.x * PLAN_NT;
+    const int gt = blockIdx.x * NT + tid, gn = gridDim.x * NT;
     if (p.slot_map) {
-        for (int r = gt; r < p.n_rows; r += gn) {
-            int slot = -1, pos = -1;
-            if (r < described) {
-                const int b = m5_upper(row_pre, B, r);
-                pos = p.keep_len[b] + (r - row_pre[b]);
-                const int page = pos >> shift, have = m5_pages(p.seq_len[b], shift);
-                const int id = page < have ? p.block_table[(int64_t)b * p.table_rs + page] : allocation(take_pre[b] + (page - have));
-                if (m5_block(id, p.n_blocks) >= 0) slot = (id << shift) + (pos & ((1 << shift) - 1));
+        constexpr int U = 4;
+        int top = 1;
+        while (2 * top < B) top *= 2;
+        for (int64_t r0 = gt; r0 < p.n_rows; r0 += (int64_t)U * gn) {
+            int b[U], pos[U], id[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) b[u] = 0;
+            for (int s = top; s; s >>= 1)                    // the last request that starts at or before the row
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int mid = b[u] + s;
+                    if (mid < B && row_pre[min(mid, B)] <= r0 + (int64_t)u * gn) b[u] = mid;
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + (int64_t)u * gn;
+                pos[u] = id[u] = -1;
+                if (r < described) {
+                    pos[u] = keep[b[u]] + ((int)r - row_pre[b[u]]);
+                    const int page = pos[u] >> shift, h = have[b[u]];
+                    id[u] = page < h ? p.block_table[(int64_t)b[u] * p.table_rs + page] : allocation(take_pre[b[u]] + (page - h));
+                }
             }
-            p.slot_map[r] = slot;
-            p.positions[r] = pos;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + (int64_t)u * gn;
+                if (r >= p.n_rows) break;
+                p.slot_map[r] = m5_block(id[u], p.n_blocks) >= 0 ? (id[u] << shift) + (pos[u] & ((1 << shift) - 1)) : -1;
+                p.positions[r] = pos[u];
+            }
         }
     }
     for (int a = gt; a < taken; a += gn) {
         const int b = m5_upper(take_pre, B, a);
-        p.block_table[(int64_t)b * p.table_rs + m5_pages(p.seq_len[b], shift) + (a - take_pre[b])] = allocation(a);
+        p.block_table[(int64_t)b * p.table_rs + have[b] + (a - take_pre[b])] = allocation(a);
     }
     for (int i = taken + gt; i < given; i += gn) p.free_blocks[m5_plan_push(i, given, n_free)] = returned(i);
     if (blockIdx.x == 0)
-        for (int b = tid; b <= B; b += PLAN_NT) p.q_start[b] = row_pre[b];
+        for (int b = tid; b <= B; b += NT) p.q_start[b] = row_pre[b];
 
-    __syncthreads();                                         // this workgroup has read all that it will of seq_len and the state
-    if (tid == 0)
-        last = gridDim.x == 1 ||
-               __hip_atomic_fetch_add(&p.state[M5_PST_ROWS + 1], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    // This workgroup has read all that it will of seq_len and the state (every load has been used or is waited for here): no cache has to
+    // be written back for the others to know, so the ticket is a relaxed one.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) last = gridDim.x == 1 || __hip_atomic_fetch_add(&p.state[M5_PST_ROWS + 1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
     __syncthreads();
     if (!last) return;
     if (ok)
-        for (int b = tid; b < B; b += PLAN_NT) p.seq_len[b] = p.keep_len[b] + p.new_len[b];
+        for (int b = tid; b < B; b += NT) p.seq_len[b] = keep[b] + (row_pre[b + 1] - row_pre[b]);
     if (tid == 0) {
         p.state[M5_PST_FREE] = n_free + given - taken;
         p.state[M5_PST_STATUS] = status;
         p.state[M5_PST_ROWS] = described;
         p.state[M5_PST_ROWS + 1] = 0;
     }
+}
+
+template <int NT>
+int launch_plan(const M5PagedPlanArgs& a, int shift, int grid, hipStream_t s) {
+    const int lds = 5 * (a.n_seq + 1) * (int)sizeof(int);
+    if (lds > 48 * 1024 && hipFuncSetAttribute((const void*)paged_plan_kernel<NT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return M5_ERR_LAUNCH;
+    hipLaunchKernelGGL(paged_plan_kernel<NT>, dim3((unsigned)grid), dim3(NT), lds, s, a, shift);
+    M5_CHECK_LAUNCH();
+    return M5_OK;
 }
 
 // ---------------------------------------------------------------------------------------------------- m5_paged_rope_cache
@@ -261,16 +301,14 @@ extern "C" int m5_paged_plan(const M5PagedPlanArgs* a, void* stream) {
     if (a->n_seq > PLAN_MAX_SEQ || a->block_size > 1024 || ((int64_t)a->table_width << shift) > INT_MAX || ((int64_t)a->n_blocks << shift) > INT_MAX ||
         (int64_t)a->n_seq * a->table_width > INT_MAX)
         return M5_ERR_UNSUPPORTED;
-    const int lds = 3 * (a->n_seq + 1) * (int)sizeof(int);
-    if (lds > 48 * 1024 &&
-        hipFuncSetAttribute((const void*)paged_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 3 * (PLAN_MAX_SEQ + 1) * (int)sizeof(int)) != hipSuccess)
-        return M5_ERR_LAUNCH;
-    // 2048 rows or 8192 pages (more than a step changes, unless requests come and go) per workgroup
-    const int64_t rows = a->slot_map ? a->n_rows : 0, pages = (int64_t)a->n_seq * a->table_width;
-    const int64_t grid = (rows + 2047) / 2048 + ((pages < a->n_blocks ? pages : a->n_blocks) >> 13);
-    hipLaunchKernelGGL(paged_plan_kernel, dim3((unsigned)(grid < 1 ? 1 : grid > 256 ? 256 : grid)), dim3(PLAN_NT), lds, (hipStream_t)stream, *a, shift);
-    M5_CHECK_LAUNCH();
-    return M5_OK;
+    const int64_t rows = a->slot_map ? a->n_rows : 0, pages = min((int64_t)a->n_seq * a->table_width, (int64_t)a->n_blocks);
+    // A workgroup per 2048 rows (1024 requests admitted and retired, 474 thousand rows: 19.1 us; 22 / 26 / 36 with 4096 / 8192 / 16384) or, in
+    // large pools, per 512 blocks that the step might give back (20.1 us with 2048).  One workgroup alone needs no ticket: 48 requests
+    // with drafts 4.3 us a call against 4.9.
+    const int64_t work = max(rows / 2048, pages < 8192 ? 0 : pages / 512);
+    const int grid = (int)min(max(work, (int64_t)1), (int64_t)256);
+    if (a->n_seq <= 256) return launch_plan<256>(*a, shift, grid, (hipStream_t)stream);
+    return launch_plan<1024>(*a, shift, grid, (hipStream_t)stream);
 }
 
 extern "C" int m5_paged_rope_cache(int dtype, const M5PagedRopeArgs* a, void* stream) {

@@ -85,7 +85,7 @@ def _check_plan(t, pool, want, got_start, slots, pos):
         assert t["table"][b, :len(p)].tolist() == p
 
 
-@pytest.mark.parametrize("n_seq,block,rows,seed", [(1, 1, 40, 1), (5, 16, 200, 2), (67, 8, 1500, 3), (1030, 4, 9001, 4), (8192, 16, 20000, 5)])
+@pytest.mark.parametrize("n_seq,block,rows,seed", [(1, 1, 40, 1), (5, 16, 200, 2), (67, 8, 1500, 3), (1030, 4, 9001, 4), (4096, 16, 20000, 5)])
 def test_plan_random_steps(dev, n_seq, block, rows, seed):
     """Admission, growth, rejected drafts, retirement and reuse over several steps against the list definition; steps that are short
     of blocks, ask for too many rows or hold an invalid request change nothing."""

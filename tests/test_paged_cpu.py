@@ -191,7 +191,7 @@ ARG, UNSUP = -1, -3
 
 @pytest.mark.parametrize("kw,rc", [(dict(seq_len=None), ARG), (dict(q_start=None), ARG), (dict(state=None), ARG), (dict(positions=None), ARG), (dict(slot_map=None), ARG),
                                    (dict(n_seq=0), ARG), (dict(n_rows=-1), ARG), (dict(block_size=24), ARG), (dict(block_size=0), ARG), (dict(table_rs=3), ARG), (dict(n_blocks=0), ARG),
-                                   (dict(block_size=2048), UNSUP), (dict(n_seq=8193), UNSUP), (dict(n_blocks=1 << 30), UNSUP), (dict(table_width=1 << 28, table_rs=1 << 28), UNSUP)])
+                                   (dict(block_size=2048), UNSUP), (dict(n_seq=4097), UNSUP), (dict(n_blocks=1 << 30), UNSUP), (dict(table_width=1 << 28, table_rs=1 << 28), UNSUP)])
 def test_plan_refuses(kw, rc):
     from mars5_tts_amd import _lib as L
     assert L.lib.m5_paged_plan(C.byref(_plan(**kw)), None) == rc
@@ -209,7 +209,7 @@ def test_rope_cache_refuses(kw, rc):
 
 @pytest.mark.parametrize("kw,rc", [(dict(q=None), ARG), (dict(out=None), ARG), (dict(seq_len=None), ARG), (dict(n_seq=0), ARG), (dict(n_heads=3, n_kv_heads=2), ARG), (dict(window=-1), ARG),
                                    (dict(scale=0.0), ARG), (dict(scale=float("nan")), ARG), (dict(block_size=10), ARG), (dict(table_rs=2), ARG), (dict(workspace_bytes=-1), ARG),
-                                   (dict(head_dim=256), UNSUP), (dict(block_size=2048), UNSUP), (dict(n_seq=10000), UNSUP), (dict(q_rs=132), UNSUP), (dict(o_hs=68), UNSUP), (dict(k_cache=P + 4), UNSUP),
+                                   (dict(head_dim=256), UNSUP), (dict(block_size=2048), UNSUP), (dict(n_seq=4097), UNSUP), (dict(q_rs=132), UNSUP), (dict(o_hs=68), UNSUP), (dict(k_cache=P + 4), UNSUP),
                                    (dict(v_bs=1020), UNSUP), (dict(workspace=P + 8, workspace_bytes=64), UNSUP)])
 def test_attention_refuses(kw, rc):
     from mars5_tts_amd import _lib as L
