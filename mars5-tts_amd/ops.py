@@ -280,6 +280,8 @@ def nar_uniforms(args: L.NarUniformArgs, stream: Optional[int] = None) -> None:
 # the current one; `stream` (a raw handle of that device) defaults to torch's current stream there.  A decode step makes dozens of these
 # calls, each of them a few microseconds long on the GPU: the checks are written out inline, without helpers per tensor.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_plan, _rope, _attn, _verify = lib.m5_paged_plan, lib.m5_paged_rope_cache, lib.m5_paged_attention, lib.m5_draft_verify
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 _NO_DEVICE = "libmars5_hip operates on device memory only"
 _DEVICES = "the tensors of a call live on one device"
@@ -288,7 +290,7 @@ _DEVICES = "the tensors of a call live on one device"
 def _launch(fn, what: str, lead: tuple, args, idx: int, stream: Optional[int]) -> None:
     if stream is None:
         stream = _raw_stream(idx)
-    if idx == torch.cuda.current_device():
+    if idx == _current_device():
         rc = fn(*lead, args, stream)
     else:
         with torch.cuda.device(idx):
@@ -335,7 +337,7 @@ def paged_plan(seq_len: torch.Tensor, keep_len: torch.Tensor, new_len: torch.Ten
         slots, where = slot_map.data_ptr(), positions.data_ptr()
     args = L.PagedPlanArgs(seq_len.data_ptr(), keep_len.data_ptr(), new_len.data_ptr(), B, block_table.shape[1], n_blocks, block_size, n_rows,
                            block_table.data_ptr(), block_table.stride(0), free_blocks.data_ptr(), state.data_ptr(), q_start.data_ptr(), slots, where)
-    _launch(lib.m5_paged_plan, "m5_paged_plan", (), C.byref(args), idx, stream)
+    _launch(_plan, "m5_paged_plan", (), C.byref(args), idx, stream)
 
 
 def paged_rope_cache(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rope: torch.Tensor, positions: torch.Tensor, slot_map: torch.Tensor,
@@ -369,7 +371,7 @@ def paged_rope_cache(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rope: tor
         return
     args = L.PagedRopeArgs(qkv.data_ptr(), qkv.stride(0), rows, n_heads, n_kv_heads, hd, qw, kw, eps, rope.data_ptr(), rope.shape[0], rope.shape[1], interleaved,
                            positions.data_ptr(), slot_map.data_ptr(), q_out.data_ptr(), q_rs, q_hs, *k, *v, n_blocks, block_size)
-    _launch(lib.m5_paged_rope_cache, "m5_paged_rope_cache", (DT_CODE[dt],), C.byref(args), idx, stream)
+    _launch(_rope, "m5_paged_rope_cache", (DT_CODE[dt],), C.byref(args), idx, stream)
 
 
 def _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, scale, window, max_new, workspace) -> tuple:
@@ -408,7 +410,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if q.shape[0] == 0:
         return
     idx, args = _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, scale, window, max_new, workspace)
-    _launch(lib.m5_paged_attention, "m5_paged_attention", (DT_CODE[q.dtype],), C.byref(args), idx, stream)
+    _launch(_attn, "m5_paged_attention", (DT_CODE[q.dtype],), C.byref(args), idx, stream)
 
 
 def paged_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor,
@@ -452,7 +454,7 @@ def draft_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: to
         ws, ws_bytes = workspace.data_ptr(), workspace.shape[0]
     args = L.DraftVerifyArgs(target.data_ptr(), target.stride(0), q, q_rs, rows, V, B, out_tokens.shape[1], tokens.data_ptr(), row_start.data_ptr(), uniforms.data_ptr(),
                              noise.data_ptr(), noise.stride(0), out_tokens.data_ptr(), out_tokens.stride(0), n_out.data_ptr(), held, kept, ws, ws_bytes)
-    _launch(lib.m5_draft_verify, "m5_draft_verify", (DT_CODE[dt],), C.byref(args), idx, stream)
+    _launch(_verify, "m5_draft_verify", (DT_CODE[dt],), C.byref(args), idx, stream)
 
 
 def expand_tokens(tokens: torch.Tensor, n_text: int, off: torch.Tensor, vals: torch.Tensor, max_run: int,
