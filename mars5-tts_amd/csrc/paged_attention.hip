@@ -240,6 +240,9 @@ struct Few {
     static constexpr int OP_B = KS * RB, STAGE_B = 2 * OP_B, WAVE_B = 2 * STAGE_B;
     static constexpr int NF = RB / 64, ND = HD / 16;             // K fragments per key row block, feature blocks of V
     static constexpr int LDS_B = NWAVE * WAVE_B;
+    // All fragments of a stage are requested before its first product where the registers allow it (5 short requests 7.63 -> 7.58 us, a chunk beside
+    // 40 single tokens 100 -> 97); with 32 or 64 rows of 128 features they do not (64 requests with drafts 308 -> 332).
+    static constexpr bool AHEAD = ES == 4 || HD == 64 || R == 1;
     static_assert(R * 16 * HD * 4 <= WAVE_B, "the waves' results meet in their rings");
 
     // 16-byte chunk swizzles: 16 (8 for V) rows of one chunk column fall into different banks
@@ -339,18 +342,53 @@ struct Few {
                 const bool whole = there == (uint32_t)((1ull << KS) - 1) && kb + KS - 1 <= pos_min && kb >= lo_max;
                 const bool odd = !whole && clean(mine + stage * STAGE_B + OP_B, there, up, down);
                 uint32_t vis[R];
+                auto key_frag = [&](int h, int t) {
+                    const int row = h * 16 + c;
+                    return *reinterpret_cast<const uint4*>(ks + row * RB + (((4 * t + g) ^ kswz(row)) << 4));
+                };
+                auto value_frag = [&](int d) {
+                    Frag v;
+                    if constexpr (ES == 4) {
+                        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int row = 4 * g + r;
+                            w[r] = *reinterpret_cast<const uint32_t*>(vs + row * RB + (((4 * d + (c >> 2)) ^ vswz(row)) << 4) + (c & 3) * 4);
+                        }
+                    } else {
+                        uint2 half[SUB];
+#pragma unroll
+                        for (int h = 0; h < SUB; ++h) {
+                            const int row = 16 * h + 4 * g + (c >> 2);
+                            half[h] = tr_read(vs + row * RB + (((2 * d + ((c >> 1) & 1)) ^ vswz(row)) << 4) + (c & 1) * 8);
+                        }
+                        if constexpr (SUB == 2) v = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
+                        else v = half[0];
+                    }
+                    return v;
+                };
+                uint4 kf[SUB][NF];
+                Frag vf[ND];
+                if constexpr (AHEAD) {
+#pragma unroll
+                    for (int h = 0; h < SUB; ++h)
+#pragma unroll
+                        for (int t = 0; t < NF; ++t) kf[h][t] = key_frag(h, t);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) vf[d] = value_frag(d);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 f4_t s[R][SUB];
 #pragma unroll
                 for (int h = 0; h < SUB; ++h) {
 #pragma unroll
                     for (int rb = 0; rb < R; ++rb) s[rb][h] = f4_t{0.f, 0.f, 0.f, 0.f};
-                    const int row = h * 16 + c;
 #pragma unroll
                     for (int t = 0; t < NF; ++t) {
-                        const uint4 k = *reinterpret_cast<const uint4*>(ks + row * RB + (((4 * t + g) ^ kswz(row)) << 4));
+                        if constexpr (!AHEAD) kf[h][t] = key_frag(h, t);
 #pragma unroll
                         for (int rb = 0; rb < R; ++rb)
-                            if (R == 1 || rb < nrb) s[rb][h] = mma16(k, qf[rb][t], s[rb][h], T());
+                            if (R == 1 || rb < nrb) s[rb][h] = mma16(kf[h][t], qf[rb][t], s[rb][h], T());
                     }
                 }
                 Frag pf[R];
@@ -391,27 +429,10 @@ struct Few {
                 }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    Frag v;
-                    if constexpr (ES == 4) {
-                        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int row = 4 * g + r;
-                            w[r] = *reinterpret_cast<const uint32_t*>(vs + row * RB + (((4 * d + (c >> 2)) ^ vswz(row)) << 4) + (c & 3) * 4);
-                        }
-                    } else {
-                        uint2 half[SUB];
-#pragma unroll
-                        for (int h = 0; h < SUB; ++h) {
-                            const int row = 16 * h + 4 * g + (c >> 2);
-                            half[h] = tr_read(vs + row * RB + (((2 * d + ((c >> 1) & 1)) ^ vswz(row)) << 4) + (c & 1) * 8);
-                        }
-                        if constexpr (SUB == 2) v = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
-                        else v = half[0];
-                    }
+                    if constexpr (!AHEAD) vf[d] = value_frag(d);
 #pragma unroll
                     for (int rb = 0; rb < R; ++rb)
-                        if (R == 1 || rb < nrb) o[rb][d] = mma16(v, pf[rb], o[rb][d], T());
+                        if (R == 1 || rb < nrb) o[rb][d] = mma16(vf[d], pf[rb], o[rb][d], T());
                 }
                 if (odd) {
                     int at = 4 * g;
