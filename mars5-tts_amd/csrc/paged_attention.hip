@@ -41,7 +41,6 @@ constexpr int NWAVE = 4, NT = NWAVE * 64;
 constexpr int MAXP = 1024;                       // block ids of one key segment held in LDS
 constexpr int MAX_SLOTS = 4096;                  // partial results of a call, and their bytes
 constexpr int64_t MAX_SLOT_BYTES = 64 << 20;
-constexpr int MIN_UNITS = 8;                     // shortest chunk of keys, in 64s: joining costs about as much as 600 keys (5 short requests: 8.2 us; 10.2 with 4)
 constexpr int MAX_SEQ = 4096;                    // item prefix sums in LDS: 16 KB
 constexpr int IDS_B = MAXP * 4, ML_B = NWAVE * 64 * 2 * 4 + 64;
 constexpr int odd_bytes(int hd) { return NWAVE * 2 * hd * 4; }   // notes of non-finite values: per wave and feature 2 x 32 keys, or 2 x 64 shared
@@ -211,18 +210,15 @@ struct Soft {
     }
 };
 
-// one row's four features: to the output, or to the item's partial result
+// four features of a row to the output
 template <typename T, int HD>
-__device__ inline void put_row(const Launch& L, const Item& it, int row, int d, f4_t o, float m, float l) {
-    const int rho = it.rho0 + row;
-    if (it.n_parts <= 1) {
-        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);         // (NaN stays NaN)
-        typename T::storage* out = (typename T::storage*)L.a.out + (int64_t)(it.rq.r0 + L.group.div(rho)) * L.a.o_rs +
-                                   (int64_t)(it.kvh * L.group.d + rho - L.group.div(rho) * L.group.d) * L.a.o_hs + d;
-        if (l == 0.f) o = f4_t{0.f, 0.f, 0.f, 0.f};
-        if constexpr (T::EPL == 4) *reinterpret_cast<f4_t*>(out) = o * inv;
-        else *reinterpret_cast<uint2*>(out) = m5_pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    }
+__device__ inline void put_row(const Launch& L, const Item& it, int row, int d, f4_t o, float l) {
+    const int rho = it.rho0 + row, tok = L.group.div(rho);
+    const float inv = l > 0.f ? 1.0f / l : l;                // (no key seen: zeros; NaN stays NaN)
+    typename T::storage* out = (typename T::storage*)L.a.out + (int64_t)(it.rq.r0 + tok) * L.a.o_rs + (int64_t)(it.kvh * L.group.d + rho - tok * L.group.d) * L.a.o_hs + d;
+    if (l == 0.f) o = f4_t{0.f, 0.f, 0.f, 0.f};
+    if constexpr (T::EPL == 4) *reinterpret_cast<f4_t*>(out) = o * inv;
+    else *reinterpret_cast<uint2*>(out) = m5_pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
 // ------------------------------------------------------------------------------------------------------ few rows
@@ -498,7 +494,7 @@ struct Few {
                 put_part(slot + row * HD + ch * 4 + 2, sum[2], sum[3]);
                 if (ch == 0) put_part(slot + 16 * R * HD + 2 * row, m, l);
             } else {
-                put_row<T, HD>(L, it, row, ch * 4, sum, m, l);
+                put_row<T, HD>(L, it, row, ch * 4, sum, l);
             }
         }
     }
@@ -754,88 +750,111 @@ struct Many {
                 if (slot) {
                     put_part(slot + row * HD + at, v[0], v[1]);
                     put_part(slot + row * HD + at + 2, v[2], v[3]);
-                } else put_row<T, HD>(L, it, row, at, v, m, l);
+                } else put_row<T, HD>(L, it, row, at, v, l);
             }
     }
 };
 
-// The last workgroup of a tile joins its partial results: the parts are dealt to groups of threads (one thread holds four features of
-// a row), eight of them in flight per thread, and the groups meet in LDS.  The order depends on the counts alone.
+// Joins a tile's partial results: the parts are dealt to groups of threads (one thread holds four features of a row), and the groups meet in
+// LDS; I rows' features and U parts are in flight per thread (a read of a part goes to memory: about a microsecond).  The order
+// depends on the counts alone.
+template <typename T, int HD, int TR, int I, int U>
+__device__ void join_all(const Launch& L, const Item& it, unsigned char* lds) {
+    const float* first = it.first_slot;
+    const int64_t stride = it.part_stride;
+    constexpr int C4 = HD / 4;
+    const int tid = threadIdx.x, chunks = (it.rho1 - it.rho0) * C4, groups = chunks < NT ? min(NT / chunks, it.n_parts) : 1;
+    f4_t* meet = reinterpret_cast<f4_t*>(lds);               // [NT] sums, then [NT] (m, l)
+    float2* meet_ml = reinterpret_cast<float2*>(lds + NT * 16);
+    const int grp = chunks < NT ? tid / chunks : 0;
+    for (int base = 0; base < chunks; base += I * NT) {
+        int at[I];
+        bool live[I];
+        float m[I], l[I];
+        f4_t sum[I];
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            at[i] = chunks < NT ? tid - grp * chunks : base + i * NT + tid;
+            live[i] = grp < groups && at[i] < chunks && (i == 0 || chunks >= NT);
+            if (!live[i]) at[i] = 0;
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+            sum[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int k0 = min(grp, it.n_parts - 1); k0 < it.n_parts; k0 += groups * U) {
+            float2 ml[I][U];
+            f4_t v[I][U];
+#pragma unroll
+            for (int i = 0; i < I; ++i)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float* s = first + min(k0 + u * groups, it.n_parts - 1) * stride;
+                    ml[i][u] = get_part(s + TR * HD + 2 * (at[i] / C4));
+                    const float2 a = get_part(s + at[i] * 4), b = get_part(s + at[i] * 4 + 2);
+                    v[i][u] = f4_t{a.x, a.y, b.x, b.y};
+                }
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                float mn = m[i];
+#pragma unroll
+                for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[i][u].x);
+                const float use = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m[i] - use);
+                m[i] = mn;
+                l[i] *= alpha;
+                sum[i] *= alpha;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float f = k0 + u * groups < it.n_parts ? __builtin_amdgcn_exp2f(ml[i][u].x - use) : 0.f;
+                    if (f != 0.f) {                          // (a part without weight adds nothing, whatever it holds)
+                        l[i] += ml[i][u].y * f;
+                        sum[i] += v[i][u] * f;
+                    }
+                }
+            }
+        }
+        if (groups > 1) {                                    // (chunks < NT: one round, i = 0)
+            meet[tid] = sum[0];
+            meet_ml[tid] = make_float2(m[0], l[0]);
+            __syncthreads();
+            if (live[0] && grp == 0) {
+                float mn = m[0];
+                for (int g = 1; g < groups; ++g) mn = fmaxf(mn, meet_ml[g * chunks + at[0]].x);
+                const float use = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m[0] - use);
+                l[0] *= alpha;
+                sum[0] *= alpha;
+                for (int g = 1; g < groups; ++g) {
+                    const float2 o = meet_ml[g * chunks + at[0]];
+                    const float f = __builtin_amdgcn_exp2f(o.x - use);
+                    if (f != 0.f) {
+                        l[0] += o.y * f;
+                        sum[0] += meet[g * chunks + at[0]] * f;
+                    }
+                }
+                m[0] = mn;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+            if (live[i] && grp == 0) put_row<T, HD>(L, it, at[i] / C4, at[i] % C4 * 4, sum[i], l[i]);
+    }
+}
+
+// Draws the tile's ticket; the workgroup that draws the last one joins.
 template <typename T, int HD, int TR>
 __device__ void join_parts(const Launch& L, const Item& it, unsigned char* lds, int* sh_last) {
     vm_wait<0>();                                            // this thread's part is in memory,
     __syncthreads();                                         // and so is the whole workgroup's
     if (threadIdx.x == 0) {
-        int* ticket = it.ticket;
-        const int n = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int n = __hip_atomic_fetch_add(it.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *sh_last = n == it.n_parts - 1;
-        if (n == it.n_parts - 1) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);       // ready for the next call
+        if (n == it.n_parts - 1) __hip_atomic_store(it.ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);    // ready for the next call
     }
     __syncthreads();
     if (!*sh_last) return;
-    const float* first = it.first_slot;
-    const int64_t stride = it.part_stride;
-    Item whole = it;
-    whole.n_parts = 1;
-    constexpr int C4 = HD / 4, U = 8;
-    const int chunks = (it.rho1 - it.rho0) * C4, groups = chunks < NT ? min(NT / chunks, it.n_parts) : 1;
-    f4_t* meet = reinterpret_cast<f4_t*>(lds);               // [NT] sums, then [NT] (m, l)
-    float2* meet_ml = reinterpret_cast<float2*>(lds + NT * 16);
-    for (int base = 0; base < chunks; base += NT) {
-        const int at = base + (int)threadIdx.x, grp = chunks < NT ? at / chunks : 0, i = chunks < NT ? at - grp * chunks : at;
-        const bool live = grp < groups && i < chunks;
-        const int row = i / C4, ch = i % C4;
-        float m = -INFINITY, l = 0.f;
-        f4_t sum = {0.f, 0.f, 0.f, 0.f};
-        if (live)
-            for (int k0 = grp; k0 < it.n_parts; k0 += groups * U) {
-                float2 ml[U];
-                f4_t v[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int k = min(k0 + u * groups, it.n_parts - 1);
-                    const float* s = first + k * stride;
-                    ml[u] = get_part(s + TR * HD + 2 * row);
-                    const float2 a = get_part(s + row * HD + ch * 4), b = get_part(s + row * HD + ch * 4 + 2);
-                    v[u] = f4_t{a.x, a.y, b.x, b.y};
-                }
-                float mn = m;
-#pragma unroll
-                for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
-                const float use = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - use);
-                m = mn;
-                l *= alpha;
-                sum *= alpha;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const float f = k0 + u * groups < it.n_parts ? __builtin_amdgcn_exp2f(ml[u].x - use) : 0.f;
-                    if (f != 0.f) {                          // (a part without weight adds nothing, whatever it holds)
-                        l += ml[u].y * f;
-                        sum += v[u] * f;
-                    }
-                }
-            }
-        if (groups > 1) {
-            meet[threadIdx.x] = sum;
-            meet_ml[threadIdx.x] = make_float2(m, l);
-            __syncthreads();
-            if (grp == 0) {
-                float mn = m;
-                for (int g = 1; g < groups; ++g) mn = fmaxf(mn, meet_ml[g * chunks + i].x);
-                const float use = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - use);
-                l *= alpha;
-                sum *= alpha;
-                for (int g = 1; g < groups; ++g) {
-                    const float2 o = meet_ml[g * chunks + i];
-                    const float f = __builtin_amdgcn_exp2f(o.x - use);
-                    l += o.y * f;
-                    sum += meet[g * chunks + i] * f;
-                }
-                m = mn;
-            }
-        }
-        if (live && grp == 0) put_row<T, HD>(L, whole, row, ch * 4, sum, m, l);
-    }
+    if ((it.rho1 - it.rho0) * (HD / 4) < NT) join_all<T, HD, TR, 1, 4>(L, it, lds);       // several groups: few parts each
+    else if (it.n_parts <= 4) join_all<T, HD, TR, 4, 4>(L, it, lds);
+    else if (it.n_parts <= 8) join_all<T, HD, TR, 2, 8>(L, it, lds);
+    else join_all<T, HD, TR, 1, 16>(L, it, lds);
 }
 
 // inclusive sum over the lanes of a wave: DPP row shifts, then the rows' last lanes broadcast
@@ -866,7 +885,7 @@ __device__ inline Share share_of(const Launch& L, const M5Request& rq) {
 
 // Items: every (request, tile, chunk of `cu` units, kv head), numbered by request.  Up to 64 requests a wave keeps in its lanes, more lie
 // in LDS as prefix sums.
-template <int TR_FEW, int TR_MANY, int HD>
+template <int TR_FEW, int TR_MANY, int HD, int MIN_UNITS>
 struct Deal {
     int cu, total;
     M5Request mine;
@@ -896,8 +915,9 @@ struct Deal {
         cu = INT_MAX >> 7;
         if (tiles < slots) {
             const float room = min(4.f * tiles <= P ? P - tiles : (tiles <= 2.f * P ? 4.f * P - tiles : 0.5f * P), slots - tiles);
-            // a tile of u units in n parts takes about a u / n + b n (the join): no shorter than sqrt(b u / a)
-            const float least = max((float)MIN_UNITS, (MANY && slot_rows == TR_MANY ? 2.2f : 1.f) * sqrtf(units / max(tiles, 1.f)));
+            // a tile of u units in n parts takes about a u / n + b n (the join): no shorter than sqrt(b u / a) (one request of 100 thousand
+            // keys and one kv head: 45 / 39 / 37 us with 1 / 0.7 / 0.5)
+            const float least = max((float)MIN_UNITS, (MANY && slot_rows == TR_MANY ? 2.2f : 0.6f) * sqrtf(units / max(tiles, 1.f)));
             cu = (int)min(max(units * 1.0001f / room + 1.f, least), (float)(INT_MAX >> 7));
         }
     }
@@ -1005,6 +1025,9 @@ template <typename T, int HD, int R, bool MANY>
 struct Shape {
     using F = Few<T, HD, R>;
     static constexpr int TR = 16 * R, TRM = MANY ? 128 : 0;
+    // Shortest chunk of keys, in 64s.  16 bits: joining costs about as much as 600 keys (5 requests of up to 700 keys: 7.6 us; 8.8 with 4).  fp32:
+    // keys cost more (chunks of 131 rows: 49 us with 4, 54 with 8).
+    static constexpr int MIN_UNITS = T::EPL == 4 ? 4 : 8;
     static constexpr int RING_B = MANY ? (F::LDS_B > 4 * 64 * HD * 2 ? F::LDS_B : 4 * 64 * HD * 2) : F::LDS_B;
     static int lds_bytes(int n_seq) { return RING_B + IDS_B + ML_B + odd_bytes(HD) + (n_seq + 1) * 4; }
 };
@@ -1018,7 +1041,7 @@ __global__ __launch_bounds__(NT, MANY || (HD == 128 && R < 4 && T::EPL == 8) || 
     int* sh = reinterpret_cast<int*>(lds + S::RING_B + IDS_B + NWAVE * 64 * 2 * 4);
     unsigned char* odd = lds + S::RING_B + IDS_B + ML_B;
     int* pre = reinterpret_cast<int*>(odd + odd_bytes(HD));
-    Deal<S::TR, S::TRM, HD> deal;
+    Deal<S::TR, S::TRM, HD, S::MIN_UNITS> deal;
     deal.setup(L, pre, ml, sh);
     for (int id = blockIdx.x; id < deal.total; id += gridDim.x) {
         Item it;
@@ -1065,7 +1088,7 @@ int launch_as(Launch& L, int cus, hipStream_t s) {
     L.places = cus * min(160 * 1024 / lds, 2);
     const int64_t tiles = ((int64_t)L.a.n_rows * L.group.d / S::TR + L.a.n_seq) * L.a.n_kv_heads;      // upper bound
     // a workgroup for every item there can be; a workgroup takes several where that is too many
-    const int64_t chunks = (((int64_t)L.a.table_width << L.shift) + 64 * MIN_UNITS - 1) / (64 * MIN_UNITS);
+    const int64_t chunks = (((int64_t)L.a.table_width << L.shift) + 64 * S::MIN_UNITS - 1) / (64 * S::MIN_UNITS);
     const int64_t grid = L.n_few ? max(min((int64_t)4 * L.places, tiles * chunks), tiles) : tiles;
     hipLaunchKernelGGL((paged_attn_kernel<T, HD, R, MANY>), dim3((unsigned)min(grid, (int64_t)1 << 20)), dim3(NT), lds, s, L);
     M5_CHECK_LAUNCH();
