@@ -18,6 +18,7 @@
 /* Block tables, slot map, positions and row offsets of one step, from the requests' lengths, in one launch.
  * Request b holds seq_len[b] positions in ceil(seq_len / block_size) blocks (block_table row b); it keeps the first keep_len[b] of
  * them (rejected drafts and finished requests, keep 0, are given back) and adds new_len[b].  Afterwards seq_len = keep + new.
+ * keep_len may be seq_len itself (all is kept).
  *   q_start[n_seq + 1]  exclusive prefix sums of new_len: the step's rows, packed by request
  *   positions[r]        position of row r in its request;  slot_map[r] = block * block_size + offset;  rows past the last: -1
  *                       (both NULL: the rows are not described, n_rows is not looked at, e.g. a roll-back)
@@ -46,7 +47,7 @@ typedef struct {
  * rotated by rope[positions[r]] (fp32 [n_pos][n_pairs][cos, sin]): features (2i, 2i + 1) when interleaved, (i, n_pairs + i)
  * otherwise.  fp32 throughout, rounded once.  q -> q_out, k and v -> slot slot_map[r] of the caches.  A row with a slot or position
  * out of range (padding: -1) is skipped and its q_out row left as it was; slots must be distinct (two rows of one slot: either
- * row's values).  head_dim 64 or 128; 2 n_pairs <= head_dim, n_pairs % 8 == 0; pointers and strides multiples of 16 bytes. */
+ * row's values).  q_out may be the q part of qkv itself.  head_dim 64 or 128; 2 n_pairs <= head_dim, n_pairs % 8 == 0; pointers and strides multiples of 16 bytes. */
 typedef struct {
     const void* qkv; int64_t qkv_rs;
     int32_t n_rows, n_heads, n_kv_heads, head_dim;
@@ -63,11 +64,12 @@ typedef struct {
  * stands at position p = seq_len[b] - (q_start[b + 1] - r) and sees the keys max(0, p - window + 1) .. p (window 0: from 0 on); query head
  * h reads kv head h / (n_heads / n_kv_heads).  Online softmax in fp32, scores never stored.  A row that sees no key gets zeros;
  * keys on a block id out of range are not seen.  Keys past a request's length and pages behind it are never used, whatever they
- * hold.  max_new: upper bound of the new tokens of one request (speed only: it selects the tiling).
+ * hold; row offsets that do not ascend compute nothing or rows of theirs twice, inside the buffers.  max_new: upper bound of the new tokens of one request (speed only: it selects the tiling).
  * workspace (may be NULL): scratch for keys split over workgroups when there are few rows; zero-filled once by the caller,
  * left ready for the next call; calls that may run at the same time need one each; 16-byte aligned.  More bytes allow more
  * splits; m5_paged_attention_workspace tells how many bytes the largest split of these shapes uses.
- * head_dim 64 or 128; n_seq <= 4096; at most 2^30 positions per table row; pointers and strides multiples of 16 bytes. */
+ * head_dim 64 or 128; n_seq <= 4096; at most 2^30 positions per table row; strides of blocks below 64 GB, of slots below 64 MB; pointers
+ * and strides multiples of 16 bytes. */
 typedef struct {
     const void* q; int64_t q_rs, q_hs;
     const void* k_cache; int64_t k_bs, k_hs, k_ss;

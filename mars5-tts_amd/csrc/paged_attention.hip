@@ -14,7 +14,7 @@
 // (keys along the register, features along the lanes) are ds_read_b64_tr_b16, which transposes 4 x 16 blocks on the way, so the
 // cache needs no transposed copy of V.
 //
-// Work.  Lengths are device data: every workgroup scans the requests (two block reductions) and deals itself items (request, tile,
+// Work.  Lengths are device data: every workgroup scans the requests (up to 64 in a wave's lanes, without a barrier) and deals itself items (request, tile,
 // key chunk, kv head), kv head fastest, so that the workgroups of one XCD (blockIdx % 8) share a head's keys in their L2.  Keys are
 // cut into chunks of C when there are fewer tiles than the chip has places for; partial (o, m, l) of a tile's chunks meet in the
 // workspace and the workgroup that arrives last joins them in chunk order (same bits whatever the order of arrival).
@@ -62,6 +62,7 @@ struct Launch {
     int shift;
     Div group, kv;                               // query heads of a kv head; kv heads
     int places;                                  // workgroups that the chip holds at a time
+    float max_tiles;                             // tiles that ascending row offsets can make
     int n_big, n_few;                            // partial results of the largest / of few-row tiles that the workspace holds (0: keys are not split)
     float* slots; int* tickets;
     float sc2;                                   // scale * log2(e)
@@ -176,11 +177,11 @@ __device__ inline int key_block(const int* ids, int key, int ka, int kb, int shi
 }
 // What the DMA reads for a key: the 16-byte chunk `ch` of its row; outside [ka, kb) the nearest key's, on a bad page block 0's (a
 // valid address: such keys are masked).  32 x 32 + 64-bit arithmetic in 16-byte units: with 64-bit strides the addresses of a tile cost
-// as much as its softmax (8 chunks of 2048 keys of 128 features: TODO against 743 TFLOP/s).
+// as much as its softmax (8 chunks of 2048 tokens, heads of 128: 743 -> 817 TFLOP/s).
 struct RowAt { uint32_t id, off; };
 __device__ inline RowAt row_at(const int* ids, int key, int ka, int kb, int shift) {
-    const int k = min(max(key, ka), kb - 1);
-    return {(uint32_t)max(ids[k >> shift], 0), (uint32_t)k & ((1u << shift) - 1)};
+    const M5KeyAt k = m5_key_at(key, ka, kb, shift);
+    return {(uint32_t)max(ids[k.page], 0), (uint32_t)k.off};
 }
 __device__ inline const unsigned char* row_chunk(const unsigned char* base, RowAt r, uint32_t bs16, uint32_t ss16, uint32_t ch) {
     return base + (((uint64_t)r.id * bs16 + (__umul24(r.off, ss16) + ch)) << 4);
@@ -572,7 +573,8 @@ struct Many {
         const int seg = (int)min(((int64_t)(MAXP - 1) << L.shift) / KT * KT, (int64_t)1 << 30);
         const uint32_t mask = (1u << L.shift) - 1;
         // A DMA instruction reads RPI consecutive rows; pages of at least as many hold them together, so the page is wave-uniform and only
-        // the offset inside it is the lane's (constant): no vector address arithmetic in the loop (c128: TODO).
+        // the offset inside it is the lane's (constant): no vector address arithmetic in the loop (with the other
+        // savings of instructions here, 8 chunks of 2048 tokens, heads of 128: 817 -> 895 TFLOP/s; heads of 64: 664 -> 730).
         const bool one_page = mask + 1 >= RPI;
         uint32_t k_off[NJ], v_off[NJ];
 #pragma unroll
@@ -869,20 +871,6 @@ __device__ inline int wave_scan(int v) {
     return dpp_add<0x143, 0xc>(v);
 }
 
-// A request's share of the work: tiles of `tr` rows and the keys that any of its rows sees, from k0 (a multiple of 64) on, in
-// units of 64.
-struct Share { int rows, tr, tiles, k0, units; };
-template <int TR_FEW, int TR_MANY>
-__device__ inline Share share_of(const Launch& L, const M5Request& rq) {
-    Share s;
-    s.rows = (rq.r1 - rq.r0) * (int)L.group.d;
-    s.tr = TR_MANY && s.rows > TR_FEW ? TR_MANY : TR_FEW;
-    s.tiles = (s.rows + s.tr - 1) / s.tr;                    // (powers of two)
-    s.k0 = m5_key_lo(rq.len - (rq.r1 - rq.r0), L.a.window) & ~63;
-    s.units = (max(rq.len - s.k0, 0) + 63) >> 6;
-    return s;
-}
-
 // Items: every (request, tile, chunk of `cu` units, kv head), numbered by request.  Up to 64 requests a wave keeps in its lanes, more lie
 // in LDS as prefix sums.
 template <int TR_FEW, int TR_MANY, int HD, int MIN_UNITS>
@@ -893,12 +881,10 @@ struct Deal {
 
     static constexpr bool MANY = TR_MANY != 0;
     int slot_rows;                                           // rows that a slot has room for
+    bool sane;                                               // row offsets that ascend (others hold more tiles than their rows can: nothing is computed)
 
-    __device__ inline int chunks(const Share& s) const {
-        if (s.units <= cu || (MANY && s.tr > slot_rows)) return 1;
-        return (int)((uint32_t)(s.units + cu - 1) / (uint32_t)cu);
-    }
-    // How long a chunk is.  items <= units / cu + tiles, and each needs a slot.
+    __device__ inline int chunks(const M5Share& s) const { return MANY && s.tr > slot_rows ? 1 : m5_chunks(s.units, cu); }
+    // How long a chunk is (m5_chunk_units).
     //  - Few tiles (at most a quarter of the places): chunks as long as the places, once filled, allow (3 requests of 60 to 120 thousand keys:
     //    159 us in 512 items, 165 / 175 / 177 in 1024 / 1536 / 2048).
     //  - Up to two per place: four items per place, so that requests of different lengths end together (64 requests of 1 to 16 thousand
@@ -909,44 +895,45 @@ struct Deal {
     __device__ inline void length(const Launch& L, float units, float tiles) {
         units *= (float)L.kv.d;
         tiles *= (float)L.kv.d;                              // (floats: exact as far as tiles are few enough to be split)
-        const float P = (float)L.places;
         slot_rows = MANY && tiles < (float)L.n_big ? TR_MANY : TR_FEW;
-        const float slots = (float)(MANY && slot_rows == TR_MANY ? L.n_big : L.n_few);
-        cu = INT_MAX >> 7;
-        if (tiles < slots) {
-            const float room = min(4.f * tiles <= P ? P - tiles : (tiles <= 2.f * P ? 4.f * P - tiles : 0.5f * P), slots - tiles);
-            // a tile of u units in n parts takes about a u / n + b n (the join): no shorter than sqrt(b u / a) (one request of 100 thousand
-            // keys and one kv head: 45 / 39 / 37 us with 1 / 0.7 / 0.5)
-            const float least = max((float)MIN_UNITS, (MANY && slot_rows == TR_MANY ? 2.2f : 0.6f) * sqrtf(units / max(tiles, 1.f)));
-            cu = (int)min(max(units * 1.0001f / room + 1.f, least), (float)(INT_MAX >> 7));
-        }
+        const bool big = MANY && slot_rows == TR_MANY;
+        // a tile of u units in n parts takes about a u / n + b n (the join): no shorter than sqrt(b u / a) (one request of 100 thousand keys
+        // and one kv head: 45 / 39 / 37 us with 1 / 0.7 / 0.5)
+        const float least = max((float)MIN_UNITS, (big ? 2.2f : 0.6f) * sqrtf(units / max(tiles, 1.f)));
+        cu = m5_chunk_units(units, tiles, (float)L.places, (float)(big ? L.n_big : L.n_few), least);
+        sane = tiles <= L.max_tiles;
     }
     __device__ inline M5Request request(const Launch& L, int b) const {
         return m5_request(L.a.q_start[b], L.a.q_start[b + 1], L.a.seq_len[b], L.a.n_rows, (int64_t)L.a.table_width << L.shift);
     }
+    __device__ inline M5Share share(const Launch& L, const M5Request& q) const { return m5_share(q, (int)L.group.d, TR_FEW, TR_MANY, L.a.window); }
     __device__ void setup(const Launch& L, int* pre, float* red, int* sums) {
         const int B = L.a.n_seq, tid = threadIdx.x, lane = tid & 63;
         if (B <= 64) {
             mine = lane < B ? request(L, lane) : M5Request{0, 0, 0};
-            const Share s = share_of<TR_FEW, TR_MANY>(L, mine);
+            const M5Share s = share(L, mine);
             length(L, wave_sum((float)s.tiles * (float)s.units), wave_sum((float)s.tiles));
-            incl = wave_scan(s.tiles * chunks(s) * (int)L.kv.d);
+            incl = wave_scan(sane ? s.tiles * chunks(s) * (int)L.kv.d : 0);
             total = __builtin_amdgcn_readlane(incl, 63);
             return;
         }
         const int per = (B + NT - 1) / NT, b0 = min(tid * per, B), b1 = min(b0 + per, B);
         float units = 0.f, tiles = 0.f;
         for (int b = b0; b < b1; ++b) {
-            const Share s = share_of<TR_FEW, TR_MANY>(L, request(L, b));
+            const M5Share s = share(L, request(L, b));
             units += (float)s.tiles * (float)s.units;
             tiles += (float)s.tiles;
         }
         units = block_sum<NWAVE>(units, red);
         tiles = block_sum<NWAVE>(tiles, red);
         length(L, units, tiles);
+        if (!sane) {
+            total = 0;
+            return;
+        }
         int n = 0;
         for (int b = b0; b < b1; ++b) {
-            const Share s = share_of<TR_FEW, TR_MANY>(L, request(L, b));
+            const M5Share s = share(L, request(L, b));
             n += s.tiles * chunks(s) * (int)L.kv.d;
         }
         const int upto = wave_scan(n);
@@ -960,7 +947,7 @@ struct Deal {
         }
         for (int b = b0; b < b1; ++b) {
             pre[b] = base;
-            const Share s = share_of<TR_FEW, TR_MANY>(L, request(L, b));
+            const M5Share s = share(L, request(L, b));
             base += s.tiles * chunks(s) * (int)L.kv.d;
         }
         if (tid == NT - 1) pre[B] = total;
@@ -980,7 +967,7 @@ struct Deal {
             it.rq = request(L, it.b);
             at = id - __builtin_amdgcn_readfirstlane(pre[it.b]);
         }
-        const Share s = share_of<TR_FEW, TR_MANY>(L, it.rq);
+        const M5Share s = share(L, it.rq);
         const int nc = chunks(s), rest = L.kv.div(at);
         it.kvh = at - rest * (int)L.kv.d;
         const int up = nc == 1 ? rest : (int)((uint32_t)rest / (uint32_t)nc), chunk = rest - up * nc;
@@ -988,29 +975,22 @@ struct Deal {
         it.rho1 = min(it.rho0 + s.tr, s.rows);
         tr = s.tr;
         const int pos0 = it.rq.len - (it.rq.r1 - it.rq.r0);
-        const int lo = m5_key_lo(pos0 + L.group.div(it.rho0), L.a.window), hi = m5_key_hi(pos0 + L.group.div(it.rho1 - 1), it.rq.len);
-        int c0 = 0, c1 = 0;
-        if (nc > 1 && hi > lo) {
-            c0 = (int)((uint32_t)((lo - s.k0) >> 6) / (uint32_t)cu);
-            c1 = (int)((uint32_t)((hi - 1 - s.k0) >> 6) / (uint32_t)cu);
-        }
-        if (chunk < c0 || chunk > c1) return false;
-        it.n_parts = c1 - c0 + 1;
+        M5Span span;
+        if (!m5_span(s, it.rq.len, L.a.window, pos0 + L.group.div(it.rho0), pos0 + L.group.div(it.rho1 - 1), nc, cu, chunk, span)) return false;
+        it.n_parts = span.c1 - span.c0 + 1;
         if (it.n_parts > 1) {
             const int64_t size = (int64_t)slot_rows * (HD + 2);              // rows of o, then (m, l) of each
-            const int first_id = id - (chunk - c0) * (int)L.kv.d;            // (ids of a tile's chunks are n_kv_heads apart)
+            const int first_id = id - (chunk - span.c0) * (int)L.kv.d;            // (ids of a tile's chunks are n_kv_heads apart)
             it.slot = L.slots + id * size;
             it.first_slot = L.slots + first_id * size;
             it.part_stride = (int64_t)L.kv.d * size;
             it.ticket = L.tickets + first_id;
         }
-        it.ka = chunk > c0 ? s.k0 + chunk * cu * 64 : lo;
-        it.kb = chunk < c1 ? s.k0 + (chunk + 1) * cu * 64 : hi;
         it.rho0 = uniform(it.rho0);
         it.rho1 = uniform(it.rho1);
         it.kvh = uniform(it.kvh);
-        it.ka = uniform(it.ka);
-        it.kb = uniform(it.kb);
+        it.ka = uniform(span.ka);
+        it.kb = uniform(span.kb);
         it.n_parts = uniform(it.n_parts);
         it.rq.r0 = uniform(it.rq.r0);
         it.rq.r1 = uniform(it.rq.r1);
@@ -1087,6 +1067,7 @@ int launch_as(Launch& L, int cus, hipStream_t s) {
     L.slots = (float*)((char*)L.a.workspace + (int64_t)L.n_few * 4);         // (n_few is a multiple of 4)
     L.places = cus * min(160 * 1024 / lds, 2);
     const int64_t tiles = ((int64_t)L.a.n_rows * L.group.d / S::TR + L.a.n_seq) * L.a.n_kv_heads;      // upper bound
+    L.max_tiles = (float)tiles * 1.001f + 1.f;
     // a workgroup for every item there can be; a workgroup takes several where that is too many
     const int64_t chunks = (((int64_t)L.a.table_width << L.shift) + 64 * S::MIN_UNITS - 1) / (64 * S::MIN_UNITS);
     const int64_t grid = L.n_few ? max(min((int64_t)4 * L.places, tiles * chunks), tiles) : tiles;

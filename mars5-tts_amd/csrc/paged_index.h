@@ -64,3 +64,52 @@ M5_HD int m5_upper(const int* pre, int n, int v) {
     }
     return lo;
 }
+
+// ---- paged_attention: how the rows and keys of the requests are dealt out (paged_attention.hip)
+
+// A request's share of the work: its packed rows (new tokens x query heads of a kv head) in tiles of `tr`, and the keys that any of
+// them sees, from k0 (a multiple of 64) on, in units of 64.
+struct M5Share { int rows, tr, tiles, k0, units; };
+M5_HD M5Share m5_share(M5Request q, int group, int tr_few, int tr_many, int window) {
+    M5Share s;
+    s.rows = (q.r1 - q.r0) * group;
+    const bool large = tr_many && s.rows > tr_few;
+    s.tr = large ? tr_many : tr_few;
+    s.tiles = large ? (s.rows + tr_many - 1) / tr_many : (s.rows + tr_few - 1) / tr_few;        // (constants in the kernels)
+    s.k0 = m5_key_lo(q.len - (q.r1 - q.r0), window) & ~63;
+    s.units = q.len > s.k0 ? (q.len - s.k0 + 63) >> 6 : 0;
+    return s;
+}
+#define M5_UNSPLIT (1 << 24)                   /* a chunk longer than any key range (2^30 positions) */
+// Units of a chunk for `units` units of work in `tiles` tiles (both over all requests and kv heads), `places` workgroups on the chip
+// and `slots` partial results; no shorter than `least`.  Items <= units / chunk + tiles <= slots: each split item has a slot.
+M5_HD int m5_chunk_units(float units, float tiles, float places, float slots, float least) {
+    if (!(tiles < slots)) return M5_UNSPLIT;
+    float room = 4.f * tiles <= places ? places - tiles : (tiles <= 2.f * places ? 4.f * places - tiles : 0.5f * places);
+    if (room > slots - tiles) room = slots - tiles;
+    float len = units * 1.0001f / room + 1.f;  // (the sums are floats: rounded up)
+    if (len < least) len = least;
+    return len < (float)M5_UNSPLIT ? (int)len : M5_UNSPLIT;
+}
+M5_HD int m5_chunks(int units, int chunk) { return units > chunk ? (int)(((unsigned)units + (unsigned)chunk - 1) / (unsigned)chunk) : 1; }
+// Keys [ka, kb) of chunk `c` of `n` for a tile whose first and last rows stand at positions `first` and `last`: false when they see none
+// of its keys and another chunk answers for the tile (chunk 0 does if they see no key at all).  The tile's chunks are c0 .. c1.
+struct M5Span { int ka, kb, c0, c1; };
+M5_HD bool m5_span(M5Share s, int len, int window, int first, int last, int n, int chunk, int c, M5Span& r) {
+    const int lo = m5_key_lo(first, window), hi = m5_key_hi(last, len);
+    r.c0 = r.c1 = 0;
+    if (n > 1 && hi > lo) {
+        r.c0 = (int)((unsigned)((lo - s.k0) >> 6) / (unsigned)chunk);
+        r.c1 = (int)((unsigned)((hi - 1 - s.k0) >> 6) / (unsigned)chunk);
+    }
+    r.ka = c > r.c0 ? s.k0 + c * chunk * 64 : lo;
+    r.kb = c < r.c1 ? s.k0 + (c + 1) * chunk * 64 : hi;
+    return c >= r.c0 && c <= r.c1;
+}
+// What is read for a key: its page among the ids of the keys [ka, kb) and its place there; outside the range the nearest key's.
+struct M5KeyAt { int page, off; };
+M5_HD M5KeyAt m5_key_at(int key, int ka, int kb, int shift) {
+    const int k = key < ka ? ka : (key >= kb ? kb - 1 : key);
+    M5KeyAt r = {k >> shift, k & ((1 << shift) - 1)};
+    return r;
+}

@@ -317,7 +317,7 @@ def paged_plan(seq_len: torch.Tensor, keep_len: torch.Tensor, new_len: torch.Ten
     (n_seq, width), the free stack (free_blocks, state[PST_FREE]) and seq_len are brought up to date, q_start (n_seq + 1,),
     slot_map and positions (n_rows,) describe the step's rows (None: not wanted).  All int32.  state (PST_WORDS,): zero-filled once,
     then state[PST_FREE] = the number of free ids; state[PST_STATUS] != 0 afterwards: nothing was done (include/mars5_paged.h).
-    The tensors must not overlap.  One launch."""
+    keep_len may be seq_len itself (all is kept); otherwise the tensors must not overlap.  One launch."""
     idx, (B,), (n_blocks,) = seq_len.get_device(), seq_len.shape, free_blocks.shape
     assert idx >= 0, _NO_DEVICE
     assert (idx == keep_len.get_device() == new_len.get_device() == block_table.get_device() == free_blocks.get_device() == state.get_device() ==
@@ -346,7 +346,8 @@ def paged_rope_cache(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rope: tor
     """``rope_cache`` for a paged cache: qkv (n_rows, (n_heads + 2 n_kv_heads) head_dim) -> RMSNorm of every q / k head (weights fp32
     (head_dim,), None = none), rotation by rope (n_pos, n_pairs, 2) fp32 (tables.rope_table) at positions, q -> q_out
     (n_rows, n_heads, head_dim), k / v -> slot_map of the caches (n_blocks, n_kv_heads, block_size, head_dim), any strides with
-    contiguous features.  Rows of slot or position -1 are skipped; slots must be distinct.  One launch."""
+    contiguous features.  Rows of slot or position -1 are skipped; slots must be distinct; q_out may be
+    the q part of qkv itself.  One launch."""
     idx, (rows, width), dt, out_shape = qkv.get_device(), qkv.shape, qkv.dtype, q_out.shape
     hd = out_shape[2]
     assert idx >= 0, _NO_DEVICE

@@ -143,6 +143,22 @@ def test_plan_short_of_blocks_and_rollback(dev):
     assert call([0, 0, 0], [0, 0, 0]) == 0 and sorted(pool.free) == list(range(7))
 
 
+def test_plan_keeps_everything_by_the_same_tensor(dev):
+    """keep_len may be seq_len itself: every request keeps all that it holds; one workgroup and many."""
+    from mars5_tts_amd import ops
+    for B, rows in ((3, 50), (900, 40000)):
+        pool = Pool(B, 12, 12 * B, 16, 2)
+        t = pool.tensors(dev)
+        for step in range(4):
+            new = [(b * 7 + step * 11) % 40 for b in range(B)] if step < 3 else [1] * B
+            new = new if B > 3 else [9, 0, 17][:B]
+            q_start, slots, pos = _i32([7] * (B + 1), dev), _i32([7] * rows, dev), _i32([7] * rows, dev)
+            want = pool.step(pool.len[:], new, rows)
+            ops.paged_plan(t["seq_len"], t["seq_len"], _i32(new, dev), t["table"], t["free"], t["state"], 16, q_start, slots, pos)
+            torch.cuda.synchronize()
+            _check_plan(t, pool, want, q_start, slots, pos)
+
+
 def test_plan_strided_table_other_stream_and_replay(dev):
     """A table that is a slice of a wider one, the call on a stream of its own, and a captured call that is replayed with eager work in
     between: every replay continues from the state of the one before."""
@@ -247,6 +263,24 @@ def test_rope_cache(dev, dt, rows, heads, kv, hd, n_pairs, inter, norm, block):
         flat = c.permute(0, 2, 1, 3).reshape(n_blocks * block, kv, hd).cpu()
         rest = [s for s in range(n_blocks * block) if s not in live]
         assert bool((flat[rest] == 9.0).all())
+
+
+def test_rope_cache_in_place(dev):
+    """q_out may be the q part of qkv itself."""
+    from mars5_tts_amd import ops, tables
+    rope = tables.rope_table(128, 100).to(dev)
+    for dt in DTS:
+        for rows in (5, 1500):
+            qkv = torch.randn(rows, 12 * 128, generator=torch.Generator().manual_seed(3)).to(dt).to(dev)
+            pos = torch.randint(0, 100, (rows,), generator=torch.Generator().manual_seed(4)).int().to(dev)
+            slot = torch.arange(rows, dtype=torch.int32, device=dev)
+            w = torch.rand(128, generator=torch.Generator().manual_seed(5)).to(dev)
+            kc, vc, kc2, vc2 = (torch.zeros(rows // 16 + 1, 2, 16, 128, dtype=dt, device=dev) for _ in range(4))
+            q = torch.zeros(rows, 8, 128, dtype=dt, device=dev)
+            ops.paged_rope_cache(qkv, 8, 2, rope, pos, slot, q, kc, vc, q_norm=w, k_norm=w, interleaved=False)
+            ops.paged_rope_cache(qkv, 8, 2, rope, pos, slot, qkv[:, :8 * 128].view(rows, 8, 128), kc2, vc2, q_norm=w, k_norm=w, interleaved=False)
+            torch.cuda.synchronize()
+            assert torch.equal(qkv[:, :8 * 128].view(rows, 8, 128), q) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
 
 
 def test_rope_cache_matches_the_contiguous_form(dev):
@@ -395,6 +429,63 @@ def test_attention_drafts(dev, dt, heads, kv, hd, block):
 def test_attention_chunks(dev, dt, heads, kv, hd, block, nhd):
     """Prompt chunks: the first (no cached positions), odd lengths, beside single tokens; both cache orders."""
     _run_attn(dev, dt, [0, 37, 200, 90, 0], [129, 64, 1, 257, 31], heads, kv, hd, block, seed=heads + 2, nhd=nhd)
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("heads,kv,hd,block", [(6, 2, 64, 1), (2, 2, 64, 4), (4, 1, 128, 2), (3, 3, 128, 1), (5, 5, 64, 1024)])
+def test_attention_small_and_large_pages(dev, dt, heads, kv, hd, block):
+    """Pages of fewer rows than one DMA instruction reads, of one row with more pages than a segment's table holds (1024), and larger than
+    any request: single tokens and chunks."""
+    _run_attn(dev, dt, [2500, 3, 1100], [1, 2, 1], heads, kv, hd, block, seed=heads + 40)
+    _run_attn(dev, dt, [1300, 0, 700], [140, 131, 1], heads, kv, hd, block, seed=heads + 41, window=1200 if hd == 64 else 0)
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("n_seq", [63, 64, 65, 300])
+def test_attention_many_requests(dev, dt, n_seq):
+    """More requests than a wave has lanes, empty ones among them, with a chunk and without, split and not."""
+    rng = random.Random(n_seq)
+    ctx = [rng.choice([0, 1, 20, 65, 130]) for _ in range(n_seq)]
+    new = [rng.choice([0, 1, 1, 2]) for _ in range(n_seq)]
+    ctx[n_seq // 2], new[n_seq - 1], new[n_seq // 2] = 1500, 1, 1
+    _run_attn(dev, dt, ctx, new, 4, 2, 64, 16, seed=n_seq)
+    new[n_seq // 3] = 150
+    _run_attn(dev, dt, ctx, new, 4, 2, 64, 16, seed=n_seq, split=n_seq != 64)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_chunk_split_by_workspace(dev, dt, hd):
+    """A chunk with a long context beside single tokens: room for partial results of 128 rows, of few rows only, of none."""
+    from mars5_tts_amd import ops
+    c, args, ws, _ = _run_attn(dev, dt, [3000, 900, 0, 2000], [150, 1, 3, 1], 4, 2, hd, 16, seed=51)
+    first = args[6].clone()
+    n = 155
+    assert ops.paged_attention_workspace(*args, max_new=150) <= 64 << 20
+    for nbytes in (64 << 20, 5 << 20, 1 << 20, 100016, 1600, 0):
+        small = torch.zeros(max(nbytes, 16), dtype=torch.uint8, device=dev)[:nbytes]
+        for _ in range(2):
+            args[6].fill_(3.0)
+            ops.paged_attention(*args, max_new=150, workspace=small if nbytes else None)
+            torch.cuda.synchronize()
+            # both are within a few roundings to dt of the exact result (checked above for the first)
+            assert float((args[6][:n].double() - first[:n].double()).abs().max()) <= 4 * u(dt) * max(1.0, float(first[:n].double().abs().max()))
+        assert nbytes == 0 or not bool(small[:16].any())                          # the tickets are back at zero
+
+
+def test_attention_refuses_row_offsets_that_do_not_ascend(dev):
+    """Row offsets are device data: offsets that claim rows over and over compute nothing and write nothing."""
+    from mars5_tts_amd import ops
+    for B in (5, 200):
+        c = Cache([40] * B, 2, 64, torch.float16, 16, dev, 3)
+        q = torch.randn(600, 4, 64, generator=torch.Generator().manual_seed(1)).half().to(dev)
+        out = torch.full((600, 4, 64), 7.0, dtype=torch.float16, device=dev)
+        start = [0 if b % 2 == 0 else 600 for b in range(B + 1)]
+        for max_new in (1, 600):
+            ops.paged_attention(q, c.kd, c.vd, c.table_d, _i32([40] * B, dev), _i32(start, dev), out, max_new=max_new)
+            torch.cuda.synchronize()
+            assert bool((out == 7.0).all()) or max_new == 600                       # (large tiles: few enough to pass for valid, inside the buffers)
+            out.fill_(7.0)
 
 
 @pytest.mark.parametrize("dt", DTS)

@@ -26,6 +26,19 @@ int h_plan(int held, int keep, int add, int width, int shift, int* o) { return m
 int h_source(int a, int r, int f) { return m5_plan_source(a, r, f); }
 int h_push(int i, int r, int f) { return m5_plan_push(i, r, f); }
 int h_upper(const int* p, int n, int v) { return m5_upper(p, n, v); }
+void h_share(int r0, int r1, int len, int group, int few, int many, int w, int* o) {
+    M5Share s = m5_share(M5Request{r0, r1, len}, group, few, many, w);
+    o[0] = s.rows; o[1] = s.tr; o[2] = s.tiles; o[3] = s.k0; o[4] = s.units;
+}
+int h_chunk_units(float u, float t, float p, float s, float l) { return m5_chunk_units(u, t, p, s, l); }
+int h_chunks(int u, int c) { return m5_chunks(u, c); }
+int h_span(const int* s, int len, int w, int first, int last, int n, int chunk, int c, int* o) {
+    M5Span r;
+    int ok = m5_span(M5Share{s[0], s[1], s[2], s[3], s[4]}, len, w, first, last, n, chunk, c, r);
+    o[0] = r.ka; o[1] = r.kb; o[2] = r.c0; o[3] = r.c1;
+    return ok;
+}
+void h_key_at(int key, int ka, int kb, int shift, int* o) { M5KeyAt r = m5_key_at(key, ka, kb, shift); o[0] = r.page; o[1] = r.off; }
 }
 """
 BIG = [-(1 << 31), -(1 << 30), -7, -1, 0, 1, 2, 63, 64, 65, 1000, (1 << 30), (1 << 31) - 1]
@@ -39,6 +52,7 @@ def host(tmp_path_factory):
     subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=undefined", "-shared", "-fPIC", f"-I{CSRC}", str(src), "-o", str(so)], check=True)
     lib = C.CDLL(str(so))
     lib.h_request.argtypes = [C.c_int] * 4 + [C.c_longlong, C.POINTER(C.c_int)]
+    lib.h_chunk_units.argtypes = [C.c_float] * 5
     lib.h_plan.argtypes = [C.c_int] * 5 + [C.POINTER(C.c_int)]
     return lib
 
@@ -128,6 +142,62 @@ def test_prefix_search(host):
         arr = (C.c_int * len(pre))(*pre)
         for v in range(pre[-1]):
             assert host.h_upper(arr, len(pre) - 1, v) == bisect.bisect_right(pre, v) - 1
+
+
+def test_attention_items_cover_every_visible_key_once(host):
+    """Tiles x chunks of a request: every (row, key) that is to be seen lies in exactly one item of its tile, an item's keys lie inside the
+    request, a tile that sees nothing has one item, and with room for partial results the items never outnumber their slots."""
+    rng = random.Random(8)
+    o, sp = (C.c_int * 5)(), (C.c_int * 4)()
+    for case in range(300):
+        group, window = rng.choice([1, 3, 4, 16]), rng.choice([0, 0, 1, 63, 64, 200])
+        few, many = rng.choice([(16, 0), (32, 0), (64, 0), (32, 128)])
+        kv, places, slots = rng.choice([1, 2, 24]), rng.choice([8, 512]), rng.choice([0, 3, 40, 4096])
+        reqs, r0 = [], 0
+        for _ in range(rng.randrange(1, 5)):
+            new = rng.choice([0, 1, 1, 2, 5, 70])
+            reqs.append((r0, r0 + new, rng.choice([0, 1, 63, 64, 65, 300, 1500]) + rng.choice([0, new])))
+            r0 += new
+        shares = []
+        for q in reqs:
+            host.h_share(*q, group, few, many, window, o)
+            shares.append(list(o))
+            rows, tr, tiles, k0, units = o
+            assert rows == (q[1] - q[0]) * group and tiles == -(-rows // tr) and tr == (many if many and rows > few else few) and k0 % 64 == 0
+        tiles, units = kv * sum(s[2] for s in shares), kv * sum(s[2] * s[4] for s in shares)
+        chunk = host.h_chunk_units(float(units), float(tiles), float(places), float(slots), rng.choice([1.0, 4.0, 8.0]))
+        assert 1 <= chunk <= 1 << 24 and (tiles < slots or chunk == 1 << 24)
+        total = 0
+        for (a, b, ln), s in zip(reqs, shares):
+            n = host.h_chunks(s[4], chunk)
+            assert n == max(1, -(-s[4] // chunk))
+            total += kv * s[2] * n
+            for t in range(s[2]):
+                first, last = t * s[1] // group, (min((t + 1) * s[1], s[0]) - 1) // group
+                pos0 = ln - (b - a)
+                spans = []
+                for c in range(n):
+                    if host.h_span((C.c_int * 5)(*s), ln, window, pos0 + first, pos0 + last, n, chunk, c, sp):
+                        spans.append((sp[0], sp[1]))
+                        assert sp[2] <= c <= sp[3] < n
+                assert len(spans) == sp[3] - sp[2] + 1 >= 1
+                seen = [j for p in range(pos0 + first, pos0 + last + 1) for j in range(max(0, p - window + 1) if window else 0, min(p + 1, ln))]
+                lo, hi = (min(seen), max(seen) + 1) if seen else (0, 0)
+                covered = [j for ka, kb in spans for j in range(ka, kb)]
+                assert covered == list(range(lo, hi)), (reqs, window, spans, lo, hi)
+        if tiles < slots:
+            assert total <= slots, (total, slots)
+
+
+def test_what_is_read_for_a_key_stays_on_the_loaded_pages(host):
+    o = (C.c_int * 2)()
+    for shift in (0, 2, 4, 10):
+        for ka, kb in ((0, 1), (5, 6), (5, 300), (64, 128), (1000, 1023)):
+            for key in list(range(max(0, ka - 70), kb + 200, 7)) + [ka, kb - 1, kb]:
+                host.h_key_at(key, ka, kb, shift, o)
+                assert ka >> shift <= o[0] <= (kb - 1) >> shift and 0 <= o[1] < 1 << shift
+                if ka <= key < kb:
+                    assert o[0] * (1 << shift) + o[1] == key
 
 
 def test_argument_structures_match_the_header(tmp_path):
