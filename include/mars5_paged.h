@@ -64,10 +64,12 @@ typedef struct {
  * stands at position p = seq_len[b] - (q_start[b + 1] - r) and sees the keys max(0, p - window + 1) .. p (window 0: from 0 on); query head
  * h reads kv head h / (n_heads / n_kv_heads).  Online softmax in fp32, scores never stored.  A row that sees no key gets zeros;
  * keys on a block id out of range are not seen.  Keys past a request's length and pages behind it are never used, whatever they
- * hold; row offsets that do not ascend compute nothing or rows of theirs twice, inside the buffers.  max_new: upper bound of the new tokens of one request (speed only: it selects the tiling).
- * workspace (may be NULL): scratch for keys split over workgroups when there are few rows; zero-filled once by the caller,
- * left ready for the next call; calls that may run at the same time need one each; 16-byte aligned.  More bytes allow more
- * splits; m5_paged_attention_workspace tells how many bytes the largest split of these shapes uses.
+ * hold; row offsets that do not ascend compute nothing or rows of theirs twice, inside the buffers.  max_new: upper bound of the
+ * new tokens of one request (speed only: it selects the tiling).
+ * workspace (may be NULL): scratch for keys split over workgroups when there are few rows; zero-filled once by the caller, left
+ * ready for the next call of any types and shapes that is given the same bytes; calls that may run at the same time need one
+ * each; no other operator's; 16-byte aligned.  More bytes allow more splits; m5_paged_attention_workspace tells how many bytes
+ * the largest split of these shapes uses.
  * head_dim 64 or 128; n_seq <= 4096; at most 2^30 positions per table row; strides of blocks below 64 GB, of slots below 64 MB; pointers
  * and strides multiples of 16 bytes. */
 typedef struct {
@@ -92,7 +94,7 @@ typedef struct {
  *   out_tokens[b] = accepted drafts, the drawn token, then -1;  n_out[b] = their number (0 for a request without rows)
  *   keep_len[b] = seq_len[b] - (r1 - r0) + n_out[b] (both NULL: not wanted): positions that m5_paged_plan keeps in the next step
  * dtype: that of target and draft.  A request of more than out_width rows counts its first out_width rows.
- * workspace (may be NULL): M5_DRAFT_WS_BYTES per request, as for m5_paged_attention; lets a row be split over workgroups. */
+ * workspace (may be NULL): M5_DRAFT_WS_BYTES per request, kept as m5_paged_attention's; lets a row be split over workgroups. */
 #define M5_DRAFT_WS_BYTES 32
 typedef struct {
     const void* target; int64_t t_rs;

@@ -3,10 +3,10 @@
 //   o[r][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp2(scale log2(e) q[r][h] . k_j - m),   m = running maximum
 //
 // Rows.  The query heads of one kv head and the new tokens of one request are packed into rows rho = token * group + head, so every
-// key and value is read once for all of them.  A tile is 16 R rows ("few": single tokens, drafts; all types) or 128 ("many": prompt
+// key and value is read once for all of them.  A tile is 16 or 32 rows ("few": single tokens, drafts; all types) or 128 ("many": prompt
 // chunks; 16-bit).  Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T: the row is the matrix column, i.e. a lane
 // owns one row, the softmax state is lane-local, and P^T goes into the second product straight from the registers of the first.
-//   few   16x16 matrix instructions.  The waves of a workgroup take different keys (32 at a time, 16 in 32 bits) of the same rows,
+//   few   16x16 matrix instructions.  The waves of a workgroup take different keys (16 at a time, 32 of 64 features) of the same rows,
 //         each with a private ring of two stages in LDS, and meet once at the end: no barrier in the key loop.
 //   many  32x32 matrix instructions.  Each wave owns 32 rows; the waves share 64-key tiles, one barrier per tile.
 // K and V rows go from memory into LDS by DMA (global_load_lds, 16 bytes per lane; the page lookup is in the lane's address).  16-byte
@@ -39,10 +39,10 @@ namespace {
 constexpr int SCHED_MFMA = 0x8, SCHED_DS = 0x100;        // sched_group_barrier: matrix instructions, LDS reads
 constexpr int NWAVE = 4, NT = NWAVE * 64;
 constexpr int MAXP = 1024;                       // block ids of one key segment held in LDS
-constexpr int MAX_SLOTS = 4096;                  // partial results of a call, and their bytes
-constexpr int64_t MAX_SLOT_BYTES = 64 << 20;
-constexpr int MAX_SEQ = 4096;                    // item prefix sums in LDS: 16 KB
-constexpr int IDS_B = MAXP * 4, ML_B = NWAVE * 64 * 2 * 4 + 64;
+constexpr int MAX_ITEMS = 4096;                  // items of a call whose keys are split
+constexpr int64_t MAX_WORKSPACE = 64 << 20, MIN_ITEM_BYTES = 16 * (64 + 2) * 4 + 4;
+constexpr int MAX_SEQ = 4096;                    // prefix sums of items and of rows of partial results in LDS: 32 KB
+constexpr int IDS_B = MAXP * 4, ML_B = NWAVE * 32 * 2 * 4 + 64;
 constexpr int odd_bytes(int hd) { return NWAVE * 2 * hd * 4; }   // notes of non-finite values: per wave and feature 2 x 32 keys, or 2 x 64 shared
 
 // x / d for 0 <= x < 2^29: (x m) >> s with m = ceil(2^s / d), s = 29 + ceil(log2 d)
@@ -63,7 +63,7 @@ struct Launch {
     Div group, kv;                               // query heads of a kv head; kv heads
     int places;                                  // workgroups that the chip holds at a time
     float max_tiles;                             // tiles that ascending row offsets can make
-    int n_big, n_few;                            // partial results of the largest / of few-row tiles that the workspace holds (0: keys are not split)
+    int n_tickets, slot_rows;                    // items and rows of partial results that the workspace holds (0: keys are not split)
     float* slots; int* tickets;
     float sc2;                                   // scale * log2(e)
     uint32_t k_bs16, k_ss16, v_bs16, v_ss16;     // block and slot strides in 16-byte units
@@ -76,6 +76,7 @@ struct Item {
     int n_parts;                                 // partial results of this tile; more than one: this item's goes to `slot`, the tile's
     float* slot; float* first_slot;              // lie part_stride floats apart from first_slot on, and meet at `ticket`
     int64_t part_stride; int* ticket;
+    int slot_rows;                               // rows of a partial result; behind them (m, l) of each
 };
 
 // ---------------------------------------------------------------------------------------------------- small pieces
@@ -228,9 +229,9 @@ struct Few {
     using st = typename T::storage;
     static constexpr int ES = sizeof(st), RB = HD * ES;          // bytes of a row
     // Keys of a stage: 8 KB of K and V, so that two workgroups share a CU and one computes while the other starts or ends an item (one
-    // workgroup of 16 KB stages: decode_long 178 us when its items filled the chip exactly once, 211-257 in 2-4 rounds).  Not for
-    // 64 rows of 128 features (their registers allow one workgroup anyway) and fp32 (16 KB).
-    static constexpr int KS = ES == 4 || (HD == 128 && R < 4) ? 16 : 32, SUB = KS / 16;
+    // workgroup of 16 KB stages: decode_long 178 us when its items filled the chip exactly once, 211-257 in 2-4 rounds).  fp32
+    // takes the same 16 keys.
+    static constexpr int KS = ES == 4 || HD == 128 ? 16 : 32, SUB = KS / 16;
     using Frag = std::conditional_t<ES == 2 && SUB == 1, uint2, uint4>;      // a lane's keys of the second product
     static constexpr int LPR = RB / 16, RPI = 64 / LPR;          // lanes per row, rows per DMA instruction
     static constexpr int NI = KS / RPI;                          // DMA instructions of K (and of V) per stage
@@ -238,7 +239,7 @@ struct Few {
     static constexpr int NF = RB / 64, ND = HD / 16;             // K fragments per key row block, feature blocks of V
     static constexpr int LDS_B = NWAVE * WAVE_B;
     // All fragments of a stage are requested before its first product where the registers allow it (5 short requests 7.63 -> 7.58 us, a chunk beside
-    // 40 single tokens 100 -> 97); with 32 or 64 rows of 128 features they do not (64 requests with drafts 308 -> 332).
+    // 40 single tokens 100 -> 97); with 32 rows of 128 features they do not (64 requests with drafts 308 -> 332).
     static constexpr bool AHEAD = ES == 4 || HD == 64 || R == 1;
     static_assert(R * 16 * HD * 4 <= WAVE_B, "the waves' results meet in their rings");
 
@@ -470,7 +471,7 @@ struct Few {
             l += lane_xor16(l);
             l += lane_xor32(l);
             const int row = rb * 16 + c;
-            if (g == 0) { ml[(wave * 64 + row) * 2] = sm[rb].m; ml[(wave * 64 + row) * 2 + 1] = l; }
+            if (g == 0) { ml[(wave * 32 + row) * 2] = sm[rb].m; ml[(wave * 32 + row) * 2 + 1] = l; }
 #pragma unroll
             for (int d = 0; d < ND; ++d) *reinterpret_cast<f4_t*>(om + row * HD + (((4 * d + g) ^ (row & 15)) << 2)) = o[rb][d];
         }
@@ -481,19 +482,19 @@ struct Few {
             const int row = i / (HD / 4), ch = i % (HD / 4);
             float m = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < NWAVE; ++w) m = fmaxf(m, ml[(w * 64 + row) * 2]);
+            for (int w = 0; w < NWAVE; ++w) m = fmaxf(m, ml[(w * 32 + row) * 2]);
             const float use = m == -INFINITY ? 0.f : m;
             f4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < NWAVE; ++w) {
-                const float f = __builtin_amdgcn_exp2f(ml[(w * 64 + row) * 2] - use);
-                l += ml[(w * 64 + row) * 2 + 1] * f;
+                const float f = __builtin_amdgcn_exp2f(ml[(w * 32 + row) * 2] - use);
+                l += ml[(w * 32 + row) * 2 + 1] * f;
                 sum += *reinterpret_cast<const f4_t*>(reinterpret_cast<const float*>(lds + w * WAVE_B) + row * HD + ((ch ^ (row & 15)) << 2)) * f;
             }
             if (slot) {
                 put_part(slot + row * HD + ch * 4, sum[0], sum[1]);
                 put_part(slot + row * HD + ch * 4 + 2, sum[2], sum[3]);
-                if (ch == 0) put_part(slot + 16 * R * HD + 2 * row, m, l);
+                if (ch == 0) put_part(slot + it.slot_rows * HD + 2 * row, m, l);
             } else {
                 put_row<T, HD>(L, it, row, ch * 4, sum, l);
             }
@@ -742,7 +743,7 @@ struct Many {
         if (w0 + c >= w1) return;
         const int row = wave * 32 + c;
         float* slot = it.n_parts > 1 ? it.slot : nullptr;
-        if (slot && hh == 0) put_part(slot + 128 * HD + 2 * row, m, l);
+        if (slot && hh == 0) put_part(slot + it.slot_rows * HD + 2 * row, m, l);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -760,7 +761,7 @@ struct Many {
 // Joins a tile's partial results: the parts are dealt to groups of threads (one thread holds four features of a row), and the groups meet in
 // LDS; I rows' features and U parts are in flight per thread (a read of a part goes to memory: about a microsecond).  The order
 // depends on the counts alone.
-template <typename T, int HD, int TR, int I, int U>
+template <typename T, int HD, int I, int U>
 __device__ void join_all(const Launch& L, const Item& it, unsigned char* lds) {
     const float* first = it.first_slot;
     const int64_t stride = it.part_stride;
@@ -791,7 +792,7 @@ __device__ void join_all(const Launch& L, const Item& it, unsigned char* lds) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const float* s = first + min(k0 + u * groups, it.n_parts - 1) * stride;
-                    ml[i][u] = get_part(s + TR * HD + 2 * (at[i] / C4));
+                    ml[i][u] = get_part(s + it.slot_rows * HD + 2 * (at[i] / C4));
                     const float2 a = get_part(s + at[i] * 4), b = get_part(s + at[i] * 4 + 2);
                     v[i][u] = f4_t{a.x, a.y, b.x, b.y};
                 }
@@ -842,7 +843,7 @@ __device__ void join_all(const Launch& L, const Item& it, unsigned char* lds) {
 }
 
 // Draws the tile's ticket; the workgroup that draws the last one joins.
-template <typename T, int HD, int TR>
+template <typename T, int HD>
 __device__ void join_parts(const Launch& L, const Item& it, unsigned char* lds, int* sh_last) {
     vm_wait<0>();                                            // this thread's part is in memory,
     __syncthreads();                                         // and so is the whole workgroup's
@@ -853,10 +854,10 @@ __device__ void join_parts(const Launch& L, const Item& it, unsigned char* lds, 
     }
     __syncthreads();
     if (!*sh_last) return;
-    if ((it.rho1 - it.rho0) * (HD / 4) < NT) join_all<T, HD, TR, 1, 4>(L, it, lds);       // several groups: few parts each
-    else if (it.n_parts <= 4) join_all<T, HD, TR, 4, 4>(L, it, lds);
-    else if (it.n_parts <= 8) join_all<T, HD, TR, 2, 8>(L, it, lds);
-    else join_all<T, HD, TR, 1, 16>(L, it, lds);
+    if ((it.rho1 - it.rho0) * (HD / 4) < NT) join_all<T, HD, 1, 4>(L, it, lds);       // several groups: few parts each
+    else if (it.n_parts <= 4) join_all<T, HD, 4, 4>(L, it, lds);
+    else if (it.n_parts <= 8) join_all<T, HD, 2, 8>(L, it, lds);
+    else join_all<T, HD, 1, 16>(L, it, lds);
 }
 
 // inclusive sum over the lanes of a wave: DPP row shifts, then the rows' last lanes broadcast
@@ -877,31 +878,29 @@ template <int TR_FEW, int TR_MANY, int HD, int MIN_UNITS>
 struct Deal {
     int cu, total;
     M5Request mine;
-    int incl;
-
-    static constexpr bool MANY = TR_MANY != 0;
-    int slot_rows;                                           // rows that a slot has room for
+    int incl, rows_incl;                                     // (up to 64 requests: items, and rows of partial results, of this lane's and all before it)
     bool sane;                                               // row offsets that ascend (others hold more tiles than their rows can: nothing is computed)
 
-    __device__ inline int chunks(const M5Share& s) const { return MANY && s.tr > slot_rows ? 1 : m5_chunks(s.units, cu); }
+    __device__ inline int chunks(const M5Share& s) const { return m5_chunks(s.units, cu); }
+    __device__ inline int items(const Launch& L, const M5Share& s) const { return s.tiles * chunks(s) * (int)L.kv.d; }
+    __device__ inline int part_rows(const Launch& L, const M5Share& s) const { return s.units > cu ? items(L, s) * s.sr : 0; }
     // How long a chunk is (m5_chunk_units).
     //  - Few tiles (at most a quarter of the places): chunks as long as the places, once filled, allow (3 requests of 60 to 120 thousand keys:
     //    159 us in 512 items, 165 / 175 / 177 in 1024 / 1536 / 2048).
     //  - Up to two per place: four items per place, so that requests of different lengths end together (64 requests of 1 to 16 thousand
     //    keys in 512 tiles: 485 us unsplit, 395 / 346 / 328 us in about 850 / 1300 / 1700 items).
+    //    Tiles of more than 32 rows up to 2 (64 requests of 4 to 16 thousand keys and 40 rows, heads of 64 / 128: 204 / 332 us with 1, 162 / 305
+    //    with 2, 166 / 328 with 2.5, 176 / 337 with 4).
     //  - More balance by themselves, only much longer ones are split (40 requests of 300 to 3000 keys beside a chunk, 1152 tiles: 120 us
     //    unsplit, 147 with the longer third in two parts).
-    //  - 128-row tiles are split only while slots of their size suffice for all.
-    __device__ inline void length(const Launch& L, float units, float tiles) {
-        units *= (float)L.kv.d;
-        tiles *= (float)L.kv.d;                              // (floats: exact as far as tiles are few enough to be split)
-        slot_rows = MANY && tiles < (float)L.n_big ? TR_MANY : TR_FEW;
-        const bool big = MANY && slot_rows == TR_MANY;
-        // a tile of u units in n parts takes about a u / n + b n (the join): no shorter than sqrt(b u / a) (one request of 100 thousand keys
-        // and one kv head: 45 / 39 / 37 us with 1 / 0.7 / 0.5)
-        const float least = max((float)MIN_UNITS, (big ? 2.2f : 0.6f) * sqrtf(units / max(tiles, 1.f)));
-        cu = m5_chunk_units(units, tiles, (float)L.places, (float)(big ? L.n_big : L.n_few), least);
-        sane = tiles <= L.max_tiles;
+    __device__ inline void length(const Launch& L, float units, float tiles, float unit_rows, float tile_rows) {
+        const float kv = (float)L.kv.d;                      // (float sums: exact as far as tiles are few enough to be split)
+        // a tile of u units in n parts takes about a u / n + b n (the join, which grows with the rows): no shorter than sqrt(b u / a) (16 rows, one
+        // request of 100 thousand keys and one kv head: 45 / 39 / 37 us with a factor of 1 / 0.7 / 0.5)
+        const float by = 0.6f + 1.6f / 128.f * tile_rows / max(tiles, 1.f);
+        cu = m5_chunk_units(units * kv, tiles * kv, unit_rows * kv, tile_rows * kv, (float)L.places, (float)L.n_tickets, (float)L.slot_rows,
+                            max((float)MIN_UNITS, by * sqrtf(units / max(tiles, 1.f))));
+        sane = tiles * kv <= L.max_tiles;
     }
     __device__ inline M5Request request(const Launch& L, int b) const {
         return m5_request(L.a.q_start[b], L.a.q_start[b + 1], L.a.seq_len[b], L.a.n_rows, (int64_t)L.a.table_width << L.shift);
@@ -912,60 +911,72 @@ struct Deal {
         if (B <= 64) {
             mine = lane < B ? request(L, lane) : M5Request{0, 0, 0};
             const M5Share s = share(L, mine);
-            length(L, wave_sum((float)s.tiles * (float)s.units), wave_sum((float)s.tiles));
-            incl = wave_scan(sane ? s.tiles * chunks(s) * (int)L.kv.d : 0);
+            const float t = (float)s.tiles, w = t * (float)s.units;
+            length(L, wave_sum(w), wave_sum(t), wave_sum(w * (float)s.sr), wave_sum(t * (float)s.sr));
+            incl = wave_scan(sane ? items(L, s) : 0);
+            rows_incl = wave_scan(sane ? part_rows(L, s) : 0);
             total = __builtin_amdgcn_readlane(incl, 63);
             return;
         }
         const int per = (B + NT - 1) / NT, b0 = min(tid * per, B), b1 = min(b0 + per, B);
-        float units = 0.f, tiles = 0.f;
+        float units = 0.f, tiles = 0.f, unit_rows = 0.f, tile_rows = 0.f;
         for (int b = b0; b < b1; ++b) {
             const M5Share s = share(L, request(L, b));
-            units += (float)s.tiles * (float)s.units;
-            tiles += (float)s.tiles;
+            const float t = (float)s.tiles, w = t * (float)s.units;
+            tiles += t;
+            units += w;
+            tile_rows += t * (float)s.sr;
+            unit_rows += w * (float)s.sr;
         }
         units = block_sum<NWAVE>(units, red);
         tiles = block_sum<NWAVE>(tiles, red);
-        length(L, units, tiles);
+        unit_rows = block_sum<NWAVE>(unit_rows, red);
+        tile_rows = block_sum<NWAVE>(tile_rows, red);
+        length(L, units, tiles, unit_rows, tile_rows);
         if (!sane) {
             total = 0;
             return;
         }
-        int n = 0;
+        int n = 0, r = 0;
         for (int b = b0; b < b1; ++b) {
             const M5Share s = share(L, request(L, b));
-            n += s.tiles * chunks(s) * (int)L.kv.d;
+            n += items(L, s);
+            r += part_rows(L, s);
         }
-        const int upto = wave_scan(n);
-        if (lane == 63) sums[tid >> 6] = upto;
+        const int n_upto = wave_scan(n), r_upto = wave_scan(r);
+        if (lane == 63) { sums[tid >> 6] = n_upto; sums[NWAVE + (tid >> 6)] = r_upto; }
         __syncthreads();
-        int base = upto - n;
+        int base = n_upto - n, row = r_upto - r;
         total = 0;
         for (int w = 0; w < NWAVE; ++w) {
-            if (w < tid >> 6) base += sums[w];
+            if (w < tid >> 6) { base += sums[w]; row += sums[NWAVE + w]; }
             total += sums[w];
         }
         for (int b = b0; b < b1; ++b) {
             pre[b] = base;
+            pre[B + 1 + b] = row;
             const M5Share s = share(L, request(L, b));
-            base += s.tiles * chunks(s) * (int)L.kv.d;
+            base += items(L, s);
+            row += part_rows(L, s);
         }
         if (tid == NT - 1) pre[B] = total;
         __syncthreads();
     }
     // item `id`: its place in its request; false where no row of the tile sees a key of the chunk
     __device__ inline bool item(const Launch& L, const int* pre, int id, Item& it, int& tr) const {
-        int at;
+        int at, row0;                                        // place in the request; first row of its partial results
         if (L.a.n_seq <= 64) {
             it.b = __builtin_popcountll(__ballot(incl <= id));           // requests that end before it
             it.rq.r0 = __builtin_amdgcn_readlane(mine.r0, it.b);
             it.rq.r1 = __builtin_amdgcn_readlane(mine.r1, it.b);
             it.rq.len = __builtin_amdgcn_readlane(mine.len, it.b);
             at = id - (it.b ? __builtin_amdgcn_readlane(incl, it.b - 1) : 0);
+            row0 = it.b ? __builtin_amdgcn_readlane(rows_incl, it.b - 1) : 0;
         } else {
             it.b = __builtin_amdgcn_readfirstlane(m5_upper(pre, L.a.n_seq, id));
             it.rq = request(L, it.b);
             at = id - __builtin_amdgcn_readfirstlane(pre[it.b]);
+            row0 = __builtin_amdgcn_readfirstlane(pre[L.a.n_seq + 1 + it.b]);
         }
         const M5Share s = share(L, it.rq);
         const int nc = chunks(s), rest = L.kv.div(at);
@@ -979,12 +990,13 @@ struct Deal {
         if (!m5_span(s, it.rq.len, L.a.window, pos0 + L.group.div(it.rho0), pos0 + L.group.div(it.rho1 - 1), nc, cu, chunk, span)) return false;
         it.n_parts = span.c1 - span.c0 + 1;
         if (it.n_parts > 1) {
-            const int64_t size = (int64_t)slot_rows * (HD + 2);              // rows of o, then (m, l) of each
-            const int first_id = id - (chunk - span.c0) * (int)L.kv.d;            // (ids of a tile's chunks are n_kv_heads apart)
-            it.slot = L.slots + id * size;
-            it.first_slot = L.slots + first_id * size;
+            const int64_t size = (int64_t)s.sr * (HD + 2);   // rows of o, then (m, l) of each
+            const int back = (chunk - span.c0) * (int)L.kv.d;               // (the chunks of a tile are n_kv_heads items apart)
+            it.slot = L.slots + (int64_t)row0 * (HD + 2) + at * size;
+            it.first_slot = it.slot - back * size;
             it.part_stride = (int64_t)L.kv.d * size;
-            it.ticket = L.tickets + first_id;
+            it.ticket = L.tickets + (id - back);
+            it.slot_rows = s.sr;
         }
         it.rho0 = uniform(it.rho0);
         it.rho1 = uniform(it.rho1);
@@ -1009,16 +1021,16 @@ struct Shape {
     // keys cost more (chunks of 131 rows: 49 us with 4, 54 with 8).
     static constexpr int MIN_UNITS = T::EPL == 4 ? 4 : 8;
     static constexpr int RING_B = MANY ? (F::LDS_B > 4 * 64 * HD * 2 ? F::LDS_B : 4 * 64 * HD * 2) : F::LDS_B;
-    static int lds_bytes(int n_seq) { return RING_B + IDS_B + ML_B + odd_bytes(HD) + (n_seq + 1) * 4; }
+    static int lds_bytes(int n_seq) { return RING_B + IDS_B + ML_B + odd_bytes(HD) + 2 * (n_seq + 1) * 4; }
 };
 
 template <typename T, int HD, int R, bool MANY>
-__global__ __launch_bounds__(NT, MANY || (HD == 128 && R < 4 && T::EPL == 8) || (HD == 64 && R < 4) ? 2 : 1) void paged_attn_kernel(Launch L) {
+__global__ __launch_bounds__(NT, HD == 64 || T::EPL == 8 ? 2 : 1) void paged_attn_kernel(Launch L) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     using S = Shape<T, HD, R, MANY>;
     int* ids = reinterpret_cast<int*>(lds + S::RING_B);
     float* ml = reinterpret_cast<float*>(lds + S::RING_B + IDS_B);
-    int* sh = reinterpret_cast<int*>(lds + S::RING_B + IDS_B + NWAVE * 64 * 2 * 4);
+    int* sh = reinterpret_cast<int*>(lds + S::RING_B + IDS_B + ML_B - 64);
     unsigned char* odd = lds + S::RING_B + IDS_B + ML_B;
     int* pre = reinterpret_cast<int*>(odd + odd_bytes(HD));
     Deal<S::TR, S::TRM, HD, S::MIN_UNITS> deal;
@@ -1030,30 +1042,23 @@ __global__ __launch_bounds__(NT, MANY || (HD == 128 && R < 4 && T::EPL == 8) || 
         if constexpr (MANY) {
             if (tr == 128) {
                 Many<T, HD>::run(L, it, lds, ids, odd);
-                if (it.n_parts > 1) join_parts<T, HD, 128>(L, it, lds, sh);
+                if (it.n_parts > 1) join_parts<T, HD>(L, it, lds, sh);
                 __syncthreads();
                 continue;
             }
         }
         S::F::run(L, it, lds, ids, ml, odd);
-        if (it.n_parts > 1) join_parts<T, HD, S::TR>(L, it, lds, sh);
+        if (it.n_parts > 1) join_parts<T, HD>(L, it, lds, sh);
         __syncthreads();
     }
 }
 
-
-
-// The tiling for these shapes: rows of a few-row tile, or 0 for the kernel with 128-row tiles.
+// The tiling for these shapes: rows of a few-row tile, or 0 for the kernel with 128-row tiles.  From 33 rows on the large tiles are faster also
+// where they are mostly empty (64 requests of 4 to 16 thousand keys, 40 / 64 rows each, heads of 64: 162 / 167 us against 178 / 184 in tiles of
+// 32; heads of 128: 305 / 321 against 364 / 378; tiles of 64 rows were slower than either).
 int tiling(int dtype, const M5PagedAttnArgs& a) {
     const int64_t rows = (int64_t)min(max(a.max_new, 1), max(a.n_rows, 1)) * (a.n_heads / a.n_kv_heads);
-    if (rows <= 16) return 16;
-    if (rows <= 32 || dtype == M5_F32) return 32;            // (64 fp32 rows need the registers of two waves: 2 x 1000 rows 570 us against 375)
-    return rows <= 64 ? 64 : 0;
-}
-
-// partial results of `rows` rows that fit `bytes` (with a 4-byte ticket each; a multiple of 4, so that what follows the tickets is aligned)
-int slots_of(int64_t bytes, int rows, int hd) {
-    return (int)min((int64_t)MAX_SLOTS, min(bytes, MAX_SLOT_BYTES) / ((int64_t)rows * (hd + 2) * 4 + 4)) & ~3;
+    return rows <= 16 ? 16 : (rows <= 32 || dtype == M5_F32 ? 32 : 0);
 }
 
 template <typename T, int HD, int R, bool MANY>
@@ -1061,16 +1066,18 @@ int launch_as(Launch& L, int cus, hipStream_t s) {
     using S = Shape<T, HD, R, MANY>;
     const int lds = S::lds_bytes(L.a.n_seq);
     if (hipFuncSetAttribute((const void*)paged_attn_kernel<T, HD, R, MANY>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return M5_ERR_LAUNCH;
-    L.n_few = slots_of(L.a.workspace ? L.a.workspace_bytes : 0, S::TR, HD);
-    L.n_big = MANY ? (int)min((int64_t)L.n_few, min(L.a.workspace ? L.a.workspace_bytes - L.n_few * 4 : 0, MAX_SLOT_BYTES) / (128 * (HD + 2) * 4)) : L.n_few;
+    const int64_t bytes = L.a.workspace ? min(L.a.workspace_bytes, MAX_WORKSPACE) : 0, row_b = (HD + 2) * 4;
+    // The tickets' place depends on the workspace's size alone: calls of other types and shapes find them zero.  (A multiple of 16 bytes.)
+    L.n_tickets = (int)min((int64_t)MAX_ITEMS, bytes / MIN_ITEM_BYTES) & ~3;
+    L.slot_rows = (int)((bytes - L.n_tickets * 4) / row_b);
     L.tickets = (int*)L.a.workspace;
-    L.slots = (float*)((char*)L.a.workspace + (int64_t)L.n_few * 4);         // (n_few is a multiple of 4)
+    L.slots = (float*)((char*)L.a.workspace + (int64_t)L.n_tickets * 4);
     L.places = cus * min(160 * 1024 / lds, 2);
     const int64_t tiles = ((int64_t)L.a.n_rows * L.group.d / S::TR + L.a.n_seq) * L.a.n_kv_heads;      // upper bound
     L.max_tiles = (float)tiles * 1.001f + 1.f;
     // a workgroup for every item there can be; a workgroup takes several where that is too many
     const int64_t chunks = (((int64_t)L.a.table_width << L.shift) + 64 * S::MIN_UNITS - 1) / (64 * S::MIN_UNITS);
-    const int64_t grid = L.n_few ? max(min((int64_t)4 * L.places, tiles * chunks), tiles) : tiles;
+    const int64_t grid = L.n_tickets ? max(min((int64_t)4 * L.places, tiles * chunks), tiles) : tiles;
     hipLaunchKernelGGL((paged_attn_kernel<T, HD, R, MANY>), dim3((unsigned)min(grid, (int64_t)1 << 20)), dim3(NT), lds, s, L);
     M5_CHECK_LAUNCH();
     return M5_OK;
@@ -1121,13 +1128,11 @@ int launch(const M5PagedAttnArgs& a, int shift, hipStream_t s) {
     if (a.head_dim == 64) {
         if constexpr (T::id != M5_F32) {
             if (tr == 0) return launch_as<T, 64, 2, true>(L, cus, s);
-            if (tr == 64) return launch_as<T, 64, 4, false>(L, cus, s);
         }
         return tr == 16 ? launch_as<T, 64, 1, false>(L, cus, s) : launch_as<T, 64, 2, false>(L, cus, s);
     }
     if constexpr (T::id != M5_F32) {
         if (tr == 0) return launch_as<T, 128, 2, true>(L, cus, s);
-        if (tr == 64) return launch_as<T, 128, 4, false>(L, cus, s);
     }
     return tr == 16 ? launch_as<T, 128, 1, false>(L, cus, s) : launch_as<T, 128, 2, false>(L, cus, s);
 }
@@ -1139,8 +1144,7 @@ extern "C" int m5_paged_attention_workspace(int dtype, const M5PagedAttnArgs* a,
     if (rc != M5_OK) return rc;
     if (!bytes) return M5_ERR_ARG;
     const int tr = tiling(dtype, *a);
-    const int rows = tr ? tr : 128;
-    *bytes = (int64_t)slots_of(MAX_SLOT_BYTES, rows, a->head_dim) * ((int64_t)rows * (a->head_dim + 2) * 4 + 4);
+    *bytes = min((int64_t)MAX_ITEMS * ((int64_t)(tr ? tr : 128) * (a->head_dim + 2) * 4 + 4), MAX_WORKSPACE);
     return M5_OK;
 }
 

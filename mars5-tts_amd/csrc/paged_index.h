@@ -68,8 +68,8 @@ M5_HD int m5_upper(const int* pre, int n, int v) {
 // ---- paged_attention: how the rows and keys of the requests are dealt out (paged_attention.hip)
 
 // A request's share of the work: its packed rows (new tokens x query heads of a kv head) in tiles of `tr`, and the keys that any of
-// them sees, from k0 (a multiple of 64) on, in units of 64.
-struct M5Share { int rows, tr, tiles, k0, units; };
+// them sees, from k0 (a multiple of 64) on, in units of 64.  A tile's partial results take `sr` rows each.
+struct M5Share { int rows, tr, tiles, k0, units, sr; };
 M5_HD M5Share m5_share(M5Request q, int group, int tr_few, int tr_many, int window) {
     M5Share s;
     s.rows = (q.r1 - q.r0) * group;
@@ -78,16 +78,22 @@ M5_HD M5Share m5_share(M5Request q, int group, int tr_few, int tr_many, int wind
     s.tiles = large ? (s.rows + tr_many - 1) / tr_many : (s.rows + tr_few - 1) / tr_few;        // (constants in the kernels)
     s.k0 = m5_key_lo(q.len - (q.r1 - q.r0), window) & ~63;
     s.units = q.len > s.k0 ? (q.len - s.k0 + 63) >> 6 : 0;
+    s.sr = s.rows < s.tr ? (s.rows + 15) & ~15 : s.tr;
     return s;
 }
 #define M5_UNSPLIT (1 << 24)                   /* a chunk longer than any key range (2^30 positions) */
-// Units of a chunk for `units` units of work in `tiles` tiles (both over all requests and kv heads), `places` workgroups on the chip
-// and `slots` partial results; no shorter than `least`.  Items <= units / chunk + tiles <= slots: each split item has a slot.
-M5_HD int m5_chunk_units(float units, float tiles, float places, float slots, float least) {
-    if (!(tiles < slots)) return M5_UNSPLIT;
-    float room = 4.f * tiles <= places ? places - tiles : (tiles <= 2.f * places ? 4.f * places - tiles : 0.5f * places);
-    if (room > slots - tiles) room = slots - tiles;
+// Units of a chunk for `units` units of work in `tiles` tiles (both over all requests and kv heads; unit_rows, tile_rows: the same sums
+// times each request's sr), `places` workgroups on the chip, at most `items` items and `rows` rows of partial results; no shorter
+// than `least`.  A request's items number at most units / chunk + tiles, so neither limit is passed.
+M5_HD int m5_chunk_units(float units, float tiles, float unit_rows, float tile_rows, float places, float items, float rows, float least) {
+    if (!(tiles < items && tile_rows < rows)) return M5_UNSPLIT;
+    const float most = tile_rows > 32.f * tiles ? 2.f : 4.f;    // items per place; joins of large tiles cost more
+    float room = 4.f * tiles <= places ? places - tiles : (tiles <= 2.f * places ? most * places - tiles : 0.5f * places);
+    if (room < 0.5f * places) room = 0.5f * places;
+    if (room > items - tiles) room = items - tiles;
     float len = units * 1.0001f / room + 1.f;  // (the sums are floats: rounded up)
+    const float by_rows = unit_rows * 1.0001f / (rows - tile_rows) + 1.f;
+    if (len < by_rows) len = by_rows;
     if (len < least) len = least;
     return len < (float)M5_UNSPLIT ? (int)len : M5_UNSPLIT;
 }

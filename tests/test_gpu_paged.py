@@ -384,7 +384,7 @@ def _run_attn(dev, dt, ctx, new, heads, kv, hd, block, window=0, seed=0, nhd=Fal
     start = [0]
     for n in new:
         start.append(start[-1] + n)
-    ws = torch.zeros(24 << 20, dtype=torch.uint8, device=dev) if split else None
+    ws = split if torch.is_tensor(split) else (torch.zeros(24 << 20, dtype=torch.uint8, device=dev) if split else None)
     args = (q, c.kd, c.vd, c.table_d, _i32(lens, dev), _i32(start, dev), out)
     ops.paged_attention(*args, scale=scale, window=window, max_new=max(new + [1]) if max_new is None else max_new, workspace=ws, stream=stream)
     torch.cuda.synchronize()
@@ -420,7 +420,7 @@ def test_attention_single_tokens(dev, dt, heads, kv, hd, block):
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("heads,kv,hd,block", SHAPES)
 def test_attention_drafts(dev, dt, heads, kv, hd, block):
-    """A few tokens per request: the packed (token, head) rows pass one tile of 16, 32, 64 for some."""
+    """A few tokens per request: the packed (token, head) rows pass one tile of 16, 32 for some."""
     _run_attn(dev, dt, [5, 0, 63, 130, 700, 33], [5, 3, 2, 8, 4, 1], heads, kv, hd, block, seed=heads + 1)
 
 
@@ -471,6 +471,24 @@ def test_attention_chunk_split_by_workspace(dev, dt, hd):
             # both are within a few roundings to dt of the exact result (checked above for the first)
             assert float((args[6][:n].double() - first[:n].double()).abs().max()) <= 4 * u(dt) * max(1.0, float(first[:n].double().abs().max()))
         assert nbytes == 0 or not bool(small[:16].any())                          # the tickets are back at zero
+
+
+@pytest.mark.parametrize("nbytes", [64 << 20, 24 << 20, 3000064])
+def test_attention_one_workspace_for_calls_of_all_shapes(dev, nbytes):
+    """The tickets of a call are where the one before it, of another type, head size or tiling, left zeros."""
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+    calls = [(torch.float32, [3000, 900], [40, 1], 4, 2, 128), (torch.bfloat16, [5000] * 6, [1] * 6, 24, 24, 64), (torch.float16, [4000, 2500, 0], [150, 1, 70], 4, 2, 128),
+             (torch.bfloat16, [6000, 3000], [5, 2], 8, 2, 128), (torch.float16, [4000, 1000], [90, 33], 2, 2, 64), (torch.float32, [5000, 0], [1, 1], 3, 3, 64)]
+    for turn in range(2):
+        for i, (dt, ctx, new, heads, kv, hd) in enumerate(calls):
+            _run_attn(dev, dt, ctx, new, heads, kv, hd, 16, seed=61 + i, split=ws)
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_partly_filled_large_tiles(dev, dt, hd):
+    """33 to 127 packed rows over long contexts: a tile's partial results take as many rows as it has, in 16s."""
+    _run_attn(dev, dt, [4000, 2500, 3100, 700], [9, 11, 31, 16], 8, 2, hd, 16, seed=71)
 
 
 def test_attention_refuses_row_offsets_that_do_not_ascend(dev):

@@ -28,13 +28,13 @@ int h_push(int i, int r, int f) { return m5_plan_push(i, r, f); }
 int h_upper(const int* p, int n, int v) { return m5_upper(p, n, v); }
 void h_share(int r0, int r1, int len, int group, int few, int many, int w, int* o) {
     M5Share s = m5_share(M5Request{r0, r1, len}, group, few, many, w);
-    o[0] = s.rows; o[1] = s.tr; o[2] = s.tiles; o[3] = s.k0; o[4] = s.units;
+    o[0] = s.rows; o[1] = s.tr; o[2] = s.tiles; o[3] = s.k0; o[4] = s.units; o[5] = s.sr;
 }
-int h_chunk_units(float u, float t, float p, float s, float l) { return m5_chunk_units(u, t, p, s, l); }
+int h_chunk_units(float u, float t, float ur, float tr, float p, float i, float r, float l) { return m5_chunk_units(u, t, ur, tr, p, i, r, l); }
 int h_chunks(int u, int c) { return m5_chunks(u, c); }
 int h_span(const int* s, int len, int w, int first, int last, int n, int chunk, int c, int* o) {
     M5Span r;
-    int ok = m5_span(M5Share{s[0], s[1], s[2], s[3], s[4]}, len, w, first, last, n, chunk, c, r);
+    int ok = m5_span(M5Share{s[0], s[1], s[2], s[3], s[4], s[5]}, len, w, first, last, n, chunk, c, r);
     o[0] = r.ka; o[1] = r.kb; o[2] = r.c0; o[3] = r.c1;
     return ok;
 }
@@ -52,7 +52,7 @@ def host(tmp_path_factory):
     subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=undefined", "-shared", "-fPIC", f"-I{CSRC}", str(src), "-o", str(so)], check=True)
     lib = C.CDLL(str(so))
     lib.h_request.argtypes = [C.c_int] * 4 + [C.c_longlong, C.POINTER(C.c_int)]
-    lib.h_chunk_units.argtypes = [C.c_float] * 5
+    lib.h_chunk_units.argtypes = [C.c_float] * 8
     lib.h_plan.argtypes = [C.c_int] * 5 + [C.POINTER(C.c_int)]
     return lib
 
@@ -146,13 +146,13 @@ def test_prefix_search(host):
 
 def test_attention_items_cover_every_visible_key_once(host):
     """Tiles x chunks of a request: every (row, key) that is to be seen lies in exactly one item of its tile, an item's keys lie inside the
-    request, a tile that sees nothing has one item, and with room for partial results the items never outnumber their slots."""
+    request, a tile that sees nothing has one item, and with room for partial results the items and their rows stay inside it."""
     rng = random.Random(8)
-    o, sp = (C.c_int * 5)(), (C.c_int * 4)()
+    o, sp = (C.c_int * 6)(), (C.c_int * 4)()
     for case in range(300):
         group, window = rng.choice([1, 3, 4, 16]), rng.choice([0, 0, 1, 63, 64, 200])
-        few, many = rng.choice([(16, 0), (32, 0), (64, 0), (32, 128)])
-        kv, places, slots = rng.choice([1, 2, 24]), rng.choice([8, 512]), rng.choice([0, 3, 40, 4096])
+        few, many = rng.choice([(16, 0), (32, 0), (32, 128)])
+        kv, places, slots, room = rng.choice([1, 2, 24]), rng.choice([8, 512]), rng.choice([0, 3, 40, 4096]), rng.choice([64, 1000, 100000])
         reqs, r0 = [], 0
         for _ in range(rng.randrange(1, 5)):
             new = rng.choice([0, 1, 1, 2, 5, 70])
@@ -162,22 +162,26 @@ def test_attention_items_cover_every_visible_key_once(host):
         for q in reqs:
             host.h_share(*q, group, few, many, window, o)
             shares.append(list(o))
-            rows, tr, tiles, k0, units = o
+            rows, tr, tiles, k0, units, sr = o
+            assert sr % 16 == 0 and min(rows, tr) <= sr <= tr
             assert rows == (q[1] - q[0]) * group and tiles == -(-rows // tr) and tr == (many if many and rows > few else few) and k0 % 64 == 0
         tiles, units = kv * sum(s[2] for s in shares), kv * sum(s[2] * s[4] for s in shares)
-        chunk = host.h_chunk_units(float(units), float(tiles), float(places), float(slots), rng.choice([1.0, 4.0, 8.0]))
-        assert 1 <= chunk <= 1 << 24 and (tiles < slots or chunk == 1 << 24)
-        total = 0
+        tile_rows, unit_rows = kv * sum(s[2] * s[5] for s in shares), kv * sum(s[2] * s[4] * s[5] for s in shares)
+        chunk = host.h_chunk_units(units, tiles, unit_rows, tile_rows, places, slots, room, rng.choice([1.0, 4.0, 8.0]))
+        fits = tiles < slots and tile_rows < room
+        assert 1 <= chunk <= 1 << 24 and (fits or chunk == 1 << 24)
+        total = part_rows = 0
         for (a, b, ln), s in zip(reqs, shares):
             n = host.h_chunks(s[4], chunk)
             assert n == max(1, -(-s[4] // chunk))
             total += kv * s[2] * n
+            part_rows += kv * s[2] * n * s[5] if n > 1 else 0
             for t in range(s[2]):
                 first, last = t * s[1] // group, (min((t + 1) * s[1], s[0]) - 1) // group
                 pos0 = ln - (b - a)
                 spans = []
                 for c in range(n):
-                    if host.h_span((C.c_int * 5)(*s), ln, window, pos0 + first, pos0 + last, n, chunk, c, sp):
+                    if host.h_span((C.c_int * 6)(*s), ln, window, pos0 + first, pos0 + last, n, chunk, c, sp):
                         spans.append((sp[0], sp[1]))
                         assert sp[2] <= c <= sp[3] < n
                 assert len(spans) == sp[3] - sp[2] + 1 >= 1
@@ -185,8 +189,10 @@ def test_attention_items_cover_every_visible_key_once(host):
                 lo, hi = (min(seen), max(seen) + 1) if seen else (0, 0)
                 covered = [j for ka, kb in spans for j in range(ka, kb)]
                 assert covered == list(range(lo, hi)), (reqs, window, spans, lo, hi)
-        if tiles < slots:
-            assert total <= slots, (total, slots)
+        if fits:
+            assert total <= slots and part_rows <= room, (total, slots, part_rows, room)
+        else:
+            assert part_rows == 0
 
 
 def test_what_is_read_for_a_key_stays_on_the_loaded_pages(host):
