@@ -41,7 +41,8 @@ constexpr int NWAVE = 4, NT = NWAVE * 64;
 constexpr int MAXP = 1024;                       // block ids of one key segment held in LDS
 constexpr int MAX_ITEMS = 4096;                  // items of a call whose keys are split
 constexpr int64_t MAX_WORKSPACE = 64 << 20, MIN_ITEM_BYTES = 16 * (64 + 2) * 4 + 4;
-constexpr int MAX_SEQ = 4096;                    // prefix sums of items and of rows of partial results in LDS: 32 KB
+constexpr int MAX_SEQ = 4096;                    // prefix sums of items (4 bytes) and of rows of partial results (2 bytes: in 16s) in LDS: 24 KB
+static_assert(MAX_WORKSPACE / (16 * (64 + 2) * 4) < 65536, "rows of partial results in 16s");
 constexpr int IDS_B = MAXP * 4, ML_B = NWAVE * 32 * 2 * 4 + 64;
 constexpr int odd_bytes(int hd) { return NWAVE * 2 * hd * 4; }   // notes of non-finite values: per wave and feature 2 x 32 keys, or 2 x 64 shared
 
@@ -954,7 +955,7 @@ struct Deal {
         }
         for (int b = b0; b < b1; ++b) {
             pre[b] = base;
-            pre[B + 1 + b] = row;
+            reinterpret_cast<uint16_t*>(pre + B + 1)[b] = (uint16_t)(row >> 4);
             const M5Share s = share(L, request(L, b));
             base += items(L, s);
             row += part_rows(L, s);
@@ -976,7 +977,7 @@ struct Deal {
             it.b = __builtin_amdgcn_readfirstlane(m5_upper(pre, L.a.n_seq, id));
             it.rq = request(L, it.b);
             at = id - __builtin_amdgcn_readfirstlane(pre[it.b]);
-            row0 = __builtin_amdgcn_readfirstlane(pre[L.a.n_seq + 1 + it.b]);
+            row0 = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint16_t*>(pre + L.a.n_seq + 1)[it.b]) << 4;
         }
         const M5Share s = share(L, it.rq);
         const int nc = chunks(s), rest = L.kv.div(at);
@@ -1021,7 +1022,7 @@ struct Shape {
     // keys cost more (chunks of 131 rows: 49 us with 4, 54 with 8).
     static constexpr int MIN_UNITS = T::EPL == 4 ? 4 : 8;
     static constexpr int RING_B = MANY ? (F::LDS_B > 4 * 64 * HD * 2 ? F::LDS_B : 4 * 64 * HD * 2) : F::LDS_B;
-    static int lds_bytes(int n_seq) { return RING_B + IDS_B + ML_B + odd_bytes(HD) + 2 * (n_seq + 1) * 4; }
+    static int lds_bytes(int n_seq) { return RING_B + IDS_B + ML_B + odd_bytes(HD) + (n_seq + 1) * 6; }
 };
 
 template <typename T, int HD, int R, bool MANY>
@@ -1075,9 +1076,13 @@ int launch_as(Launch& L, int cus, hipStream_t s) {
     L.places = cus * min(160 * 1024 / lds, 2);
     const int64_t tiles = ((int64_t)L.a.n_rows * L.group.d / S::TR + L.a.n_seq) * L.a.n_kv_heads;      // upper bound
     L.max_tiles = (float)tiles * 1.001f + 1.f;
-    // a workgroup for every item there can be; a workgroup takes several where that is too many
+    // A workgroup for every item there can be; a workgroup takes several where that is too many, and where every one has to go through a long
+    // list of requests (2000 of 100 to 1500 keys, 8000 tiles: 734 us with a workgroup each, 490 / 470 / 460 with 8 / 4 / 2 per place; 70 longer
+    // ones 117 with 8 / 4, 119 with 2).
     const int64_t chunks = (((int64_t)L.a.table_width << L.shift) + 64 * S::MIN_UNITS - 1) / (64 * S::MIN_UNITS);
-    const int64_t grid = L.n_tickets ? max(min((int64_t)4 * L.places, tiles * chunks), tiles) : tiles;
+    const int64_t most = (int64_t)4 * L.places;
+    int64_t grid = L.n_tickets ? max(min(most, tiles * chunks), tiles) : tiles;
+    if (L.a.n_seq > 64) grid = min(grid, most);
     hipLaunchKernelGGL((paged_attn_kernel<T, HD, R, MANY>), dim3((unsigned)min(grid, (int64_t)1 << 20)), dim3(NT), lds, s, L);
     M5_CHECK_LAUNCH();
     return M5_OK;
