@@ -41,7 +41,7 @@ namespace {
 
 constexpr int SCHED_MFMA = 0x8, SCHED_DS = 0x100;        // sched_group_barrier: matrix instructions, LDS reads
 constexpr int NWAVE = 4, NT = NWAVE * 64;
-constexpr int MAXP = 1024;                       // block ids of one key segment held in LDS
+constexpr int MAXP = 512;                        // block ids of one key segment held in LDS
 constexpr int MAX_ITEMS = 4096;                  // items of a call whose keys are split
 constexpr int64_t MAX_WORKSPACE = 64 << 20, MIN_ITEM_BYTES = 16 * (64 + 2) * 4 + 4;
 constexpr int MAX_SEQ = 4096;                    // prefix sums of items (4 bytes) and of rows of partial results (2 bytes: in 16s) in LDS: 24 KB
@@ -1025,7 +1025,7 @@ struct Shape {
     // keys cost more (chunks of 131 rows: 49 us with 4, 54 with 8).
     static constexpr int MIN_UNITS = T::EPL == 4 ? 4 : 8;
     static constexpr int RING_B = MANY ? (F::LDS_B > 4 * 64 * HD * 2 ? F::LDS_B : 4 * 64 * HD * 2) : F::LDS_B;
-    static int lds_bytes(int n_seq) { return RING_B + IDS_B + ML_B + odd_bytes(HD) + (n_seq + 1) * 6; }
+    static constexpr int lds_bytes(int n_seq) { return RING_B + IDS_B + ML_B + odd_bytes(HD) + (n_seq + 1) * 6; }
 };
 
 template <typename T, int HD, int R, bool MANY>
@@ -1068,6 +1068,7 @@ int tiling(int dtype, const M5PagedAttnArgs& a) {
 template <typename T, int HD, int R, bool MANY>
 int launch_as(Launch& L, int cus, hipStream_t s) {
     using S = Shape<T, HD, R, MANY>;
+    static_assert(S::lds_bytes(MAX_SEQ) <= 160 * 1024, "the largest batch's LDS");
     const int lds = S::lds_bytes(L.a.n_seq);
     if (hipFuncSetAttribute((const void*)paged_attn_kernel<T, HD, R, MANY>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return M5_ERR_LAUNCH;
     const int64_t bytes = L.a.workspace ? min(L.a.workspace_bytes, MAX_WORKSPACE) : 0, row_b = (HD + 2) * 4;

@@ -453,6 +453,19 @@ def test_attention_many_requests(dev, dt, n_seq):
     _run_attn(dev, dt, ctx, new, 4, 2, 64, 16, seed=n_seq, split=n_seq != 64)
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_the_longest_list_of_requests(dev, dt, hd):
+    """4096 requests: their prefix sums and the rings of every variant fit the LDS together."""
+    ctx, new = [0] * 4096, [0] * 4096
+    for i, b in enumerate(range(0, 4096, 117)):
+        ctx[b], new[b] = 40 * i, 1 + i % 2
+    new[4095] = 1
+    _run_attn(dev, dt, ctx, new, 2, 1, hd, 16, seed=81)
+    new[2000] = 70
+    _run_attn(dev, dt, ctx, new, 2, 1, hd, 16, seed=82)
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_attention_chunk_split_by_workspace(dev, dt, hd):
