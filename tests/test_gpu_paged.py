@@ -961,3 +961,59 @@ def test_speculative_serving_run(dev):
     assert total > 9 * B                                                         # some drafts were accepted
     ops.paged_plan(t["seq_len"], _i32([0] * B, dev), _i32([0] * B, dev), t["table"], t["free"], t["state"], block, q_start)
     assert sorted(t["free"].tolist()) == list(range(n_blocks)) and int(t["state"][L.PST_FREE]) == n_blocks
+
+
+def test_recorded_step_equals_the_calls(dev):
+    """A whole step recorded as a stage plan: run from C, then captured into a graph and replayed, beside the same calls one by one; the
+    keep_len that verification writes is the next step's, so every step depends on the ones before."""
+    from mars5_tts_amd import _lib as L, ops
+    B, block, width, n_blocks, H, kv, hd, V, M = 5, 4, 16, 64, 4, 2, 64, 500, 3
+    rows = B * M
+    g = torch.Generator().manual_seed(9)
+    qkv = torch.randn(rows, (H + 2 * kv) * hd, generator=g).bfloat16().to(dev)
+    rope = torch.randn(width * block, hd // 2, 2, generator=g).to(dev)
+    target, draft = (torch.softmax(torch.randn(rows, V, generator=g) * 2, -1).to(dev) for _ in range(2))
+    tokens = torch.randint(0, V, (rows,), generator=g).to(dev)
+    tokens[1::2] = target[0::2].argmax(-1)[:tokens[1::2].shape[0]]               # some drafts are likely ones
+    uni, noise = torch.rand(rows, generator=g).to(dev), torch.empty(B, V).exponential_(generator=g).to(dev)
+    new = _i32([M] * B, dev)
+
+    def fresh():
+        t = dict(seq_len=_i32([0] * B, dev), keep=_i32([0] * B, dev), table=torch.zeros(B, width, dtype=torch.int32, device=dev),
+                 free=torch.arange(n_blocks, dtype=torch.int32, device=dev), state=torch.zeros(L.PST_WORDS, dtype=torch.int32, device=dev),
+                 q_start=_i32([0] * (B + 1), dev), slots=_i32([0] * rows, dev), pos=_i32([0] * rows, dev),
+                 q=torch.zeros(rows, H, hd, dtype=torch.bfloat16, device=dev), out=torch.zeros(rows, H, hd, dtype=torch.bfloat16, device=dev),
+                 k=torch.zeros(n_blocks, kv, block, hd, dtype=torch.bfloat16, device=dev), v=torch.zeros(n_blocks, kv, block, hd, dtype=torch.bfloat16, device=dev),
+                 out_tokens=torch.zeros(B, M, dtype=torch.int64, device=dev), n_out=_i32([0] * B, dev), ws=torch.zeros(1 << 20, dtype=torch.uint8, device=dev),
+                 vs=torch.zeros(B * L.DRAFT_WS_BYTES, dtype=torch.uint8, device=dev))
+        t["state"][L.PST_FREE] = n_blocks
+        return t
+
+    def step(t):
+        ops.paged_plan(t["seq_len"], t["keep"], new, t["table"], t["free"], t["state"], block, t["q_start"], t["slots"], t["pos"])
+        ops.paged_rope_cache(qkv, H, kv, rope, t["pos"], t["slots"], t["q"], t["k"], t["v"])
+        ops.paged_attention(t["q"], t["k"], t["v"], t["table"], t["seq_len"], t["q_start"], t["out"], max_new=M, workspace=t["ws"])
+        ops.draft_verify(target, draft, tokens, t["q_start"], uni, noise, t["out_tokens"], t["n_out"], seq_len=t["seq_len"], keep_len=t["keep"], workspace=t["vs"])
+
+    one, two, three = fresh(), fresh(), fresh()
+    plan2, plan3 = ops.StagePlan("ar_decode_step"), ops.StagePlan("ar_decode_step")
+    with plan2.recording():
+        step(two)
+    with plan3.recording():
+        step(three)
+    assert plan2.n_ops == plan3.n_ops == 4 and int(two["n_out"].sum()) == 0
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        plan3.run(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(8):
+        step(one)
+        plan2.run()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(one["state"][L.PST_STATUS]) == 0 and int(one["n_out"].min()) >= 1
+        for name in one:
+            assert torch.equal(one[name], two[name]) and torch.equal(one[name], three[name]), (i, name)
+    assert int(one["seq_len"].max()) > 8
