@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct as _struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # M5_HIP_TOOLS=1 (set by tools/*.py before importing the package) loads the tools build of the same sources:
@@ -183,6 +184,16 @@ class DraftVerifyArgs(C.Structure):
                 ("tokens", vp), ("row_start", vp), ("uniforms", vp), ("noise", vp), ("noise_rs", i64),
                 ("out_tokens", vp), ("out_rs", i64), ("n_out", vp), ("seq_len", vp), ("keep_len", vp),
                 ("workspace", vp), ("workspace_bytes", i64)]
+
+
+def packed(cls):
+    """``cls(*values)``, all fields given (pointers as integers), in less than half the time: packed at once instead of set field by
+    field.  A value that does not fit its field raises struct.error."""
+    code = {vp: "P", i64: "q", i32: "i", f32: "f"}
+    fmt = _struct.Struct("@" + "".join(code[t] for _, t in cls._fields_) + "0q")        # (native alignment, whole 8 bytes at the end)
+    assert fmt.size == C.sizeof(cls), cls.__name__
+    pack, take = fmt.pack, cls.from_buffer_copy
+    return lambda *values: take(pack(*values))
 
 
 PST_FREE, PST_STATUS, PST_ROWS, PST_WORDS = 0, 1, 2, 8

@@ -282,6 +282,7 @@ def nar_uniforms(args: L.NarUniformArgs, stream: Optional[int] = None) -> None:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _plan, _rope, _attn, _verify = lib.m5_paged_plan, lib.m5_paged_rope_cache, lib.m5_paged_attention, lib.m5_draft_verify
+_plan_args, _rope_args, _attn_args, _verify_args = (L.packed(c) for c in (L.PagedPlanArgs, L.PagedRopeArgs, L.PagedAttnArgs, L.DraftVerifyArgs))
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 _NO_DEVICE = "libmars5_hip operates on device memory only"
 _DEVICES = "the tensors of a call live on one device"
@@ -328,15 +329,15 @@ def paged_plan(seq_len: torch.Tensor, keep_len: torch.Tensor, new_len: torch.Ten
             q_start.is_contiguous()), "contiguous tensors (a table's rows may lie apart)"
     assert block_table.dim() == 2 and block_table.shape[0] == B and block_table.stride(1) == 1, "block_table: (n_seq, width)"
     assert (slot_map is None) == (positions is None), "slot_map and positions go together"
-    n_rows, slots, where = 0, None, None
+    n_rows = slots = where = 0
     if slot_map is not None:
         (n_rows,) = slot_map.shape
         assert n_rows > 0, "slot_map of no rows: pass None"
         assert idx == slot_map.get_device() == positions.get_device(), _DEVICES
         assert slot_map.dtype == positions.dtype == _I32 and positions.shape == (n_rows,) and slot_map.is_contiguous() and positions.is_contiguous(), "slot_map, positions: (n_rows,) int32"
         slots, where = slot_map.data_ptr(), positions.data_ptr()
-    args = L.PagedPlanArgs(seq_len.data_ptr(), keep_len.data_ptr(), new_len.data_ptr(), B, block_table.shape[1], n_blocks, block_size, n_rows,
-                           block_table.data_ptr(), block_table.stride(0), free_blocks.data_ptr(), state.data_ptr(), q_start.data_ptr(), slots, where)
+    args = _plan_args(seq_len.data_ptr(), keep_len.data_ptr(), new_len.data_ptr(), B, block_table.shape[1], n_blocks, block_size, n_rows,
+                      block_table.data_ptr(), block_table.stride(0), free_blocks.data_ptr(), state.data_ptr(), q_start.data_ptr(), slots, where)
     _launch(_plan, "m5_paged_plan", (), C.byref(args), idx, stream)
 
 
@@ -361,7 +362,7 @@ def paged_rope_cache(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rope: tor
     q_rs, q_hs, q1 = q_out.stride()
     assert q1 == 1, "q_out: features are contiguous"
     n_blocks, block_size, k, v = _caches(k_cache, v_cache, dt, n_kv_heads, hd)
-    qw = kw = None
+    qw = kw = 0
     if q_norm is not None:
         assert q_norm.dtype == _F32 and q_norm.shape == (hd,) and q_norm.is_contiguous() and q_norm.get_device() == idx, "q_norm: (head_dim,) fp32"
         qw = q_norm.data_ptr()
@@ -370,8 +371,8 @@ def paged_rope_cache(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rope: tor
         kw = k_norm.data_ptr()
     if rows == 0:
         return
-    args = L.PagedRopeArgs(qkv.data_ptr(), qkv.stride(0), rows, n_heads, n_kv_heads, hd, qw, kw, eps, rope.data_ptr(), rope.shape[0], rope.shape[1], interleaved,
-                           positions.data_ptr(), slot_map.data_ptr(), q_out.data_ptr(), q_rs, q_hs, *k, *v, n_blocks, block_size)
+    args = _rope_args(qkv.data_ptr(), qkv.stride(0), rows, n_heads, n_kv_heads, hd, qw, kw, eps, rope.data_ptr(), rope.shape[0], rope.shape[1], interleaved,
+                      positions.data_ptr(), slot_map.data_ptr(), q_out.data_ptr(), q_rs, q_hs, *k, *v, n_blocks, block_size)
     _launch(_rope, "m5_paged_rope_cache", (DT_CODE[dt],), C.byref(args), idx, stream)
 
 
@@ -395,9 +396,9 @@ def _paged_attn_args(q, k_cache, v_cache, block_table, seq_len, q_start, out, sc
     if workspace is not None:
         assert workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous() and workspace.get_device() == idx, "workspace: zero-filled uint8 bytes"
         ws, ws_bytes = workspace.data_ptr(), workspace.shape[0]
-    return idx, L.PagedAttnArgs(q.data_ptr(), q_rs, q_hs, *k, *v, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], n_blocks, block_size,
-                                B, rows, rows if max_new is None else max_new, heads, kv, hd, window, seq_len.data_ptr(), q_start.data_ptr(),
-                                hd ** -0.5 if scale is None else scale, out.data_ptr(), o_rs, o_hs, ws, ws_bytes)
+    return idx, _attn_args(q.data_ptr(), q_rs, q_hs, *k, *v, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], n_blocks, block_size,
+                           B, rows, rows if max_new is None else max_new, heads, kv, hd, window, seq_len.data_ptr(), q_start.data_ptr(),
+                           hd ** -0.5 if scale is None else scale, out.data_ptr(), o_rs, o_hs, ws, ws_bytes)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor,
@@ -453,8 +454,8 @@ def draft_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: to
     if workspace is not None:
         assert workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous() and workspace.get_device() == idx, "workspace: zero-filled uint8 bytes"
         ws, ws_bytes = workspace.data_ptr(), workspace.shape[0]
-    args = L.DraftVerifyArgs(target.data_ptr(), target.stride(0), q, q_rs, rows, V, B, out_tokens.shape[1], tokens.data_ptr(), row_start.data_ptr(), uniforms.data_ptr(),
-                             noise.data_ptr(), noise.stride(0), out_tokens.data_ptr(), out_tokens.stride(0), n_out.data_ptr(), held, kept, ws, ws_bytes)
+    args = _verify_args(target.data_ptr(), target.stride(0), q, q_rs, rows, V, B, out_tokens.shape[1], tokens.data_ptr(), row_start.data_ptr(), uniforms.data_ptr(),
+                        noise.data_ptr(), noise.stride(0), out_tokens.data_ptr(), out_tokens.stride(0), n_out.data_ptr(), held, kept, ws, ws_bytes)
     _launch(_verify, "m5_draft_verify", (DT_CODE[dt],), C.byref(args), idx, stream)
 
 

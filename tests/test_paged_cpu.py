@@ -144,6 +144,17 @@ def test_prefix_search(host):
             assert host.h_upper(arr, len(pre) - 1, v) == bisect.bisect_right(pre, v) - 1
 
 
+def test_packed_structures_equal_the_field_by_field_ones():
+    from mars5_tts_amd import _lib as L
+    import struct
+    for cls in (L.PagedPlanArgs, L.PagedRopeArgs, L.PagedAttnArgs, L.DraftVerifyArgs):
+        values = [0.25 if t is L.f32 else (1 << 40) + i if t in (L.vp, L.i64) else i - 3 for i, (_, t) in enumerate(cls._fields_)]
+        assert bytes(L.packed(cls)(*values)) == bytes(cls(*values))
+        values[[t for _, t in cls._fields_].index(L.i32)] = 1 << 31
+        with pytest.raises(struct.error):
+            L.packed(cls)(*values)
+
+
 def test_attention_items_cover_every_visible_key_once(host):
     """Tiles x chunks of a request: every (row, key) that is to be seen lies in exactly one item of its tile, an item's keys lie inside the
     request, a tile that sees nothing has one item, and with room for partial results the items and their rows stay inside it."""
