@@ -199,6 +199,11 @@ __device__ inline void put_part(float* p, float a, float b) {
     __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), (unsigned long long)__float_as_uint(a) | (unsigned long long)__float_as_uint(b) << 32,
                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// four of them, 16-byte aligned, by one store of that scope (neighbouring lanes fill whole lines: half-filled ones cost the memory twice);
+// waited for like the others (the wait state: the data registers may be written right behind)
+__device__ inline void put_part4(float* p, f4_t v) {
+    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" :: "v"(p), "v"(v) : "memory");
+}
 __device__ inline float2 get_part(const float* p) {
     const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
@@ -496,8 +501,7 @@ struct Few {
                 sum += *reinterpret_cast<const f4_t*>(reinterpret_cast<const float*>(lds + w * WAVE_B) + row * HD + ((ch ^ (row & 15)) << 2)) * f;
             }
             if (slot) {
-                put_part(slot + row * HD + ch * 4, sum[0], sum[1]);
-                put_part(slot + row * HD + ch * 4 + 2, sum[2], sum[3]);
+                put_part4(slot + row * HD + ch * 4, sum);
                 if (ch == 0) put_part(slot + it.slot_rows * HD + 2 * row, m, l);
             } else {
                 put_row<T, HD>(L, it, row, ch * 4, sum, l);
@@ -742,23 +746,33 @@ struct Many {
                 if (w0 < w1 && kb <= pos_max && kb + KT > lo_min) tile(kb, stage, there, odd);
             }
         }
-        if (w0 >= w1) return;
         l += lane_xor32(l);
+        if (it.n_parts > 1) {
+            // Through LDS, so that a wave stores whole rows (64 requests of 4 to 16 thousand keys, 128 rows each, heads of 64 / 128: 191 / 366 us
+            // with a row per lane, 64 pieces of as many lines a store; 168 / 341 so).
+            __syncthreads();                                     // all waves are done with the stages
+            float* om = reinterpret_cast<float*>(lds) + wave * 32 * HD;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f4_t*>(om + c * HD + (((8 * d + 2 * q + hh) ^ (c & 7)) << 2)) = f4_t{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+            lds_wait();
+            float* slot = it.slot + (int64_t)wave * 32 * HD;
+            for (int i = lane; i < (w1 - w0) * (HD / 4); i += 64) {
+                const int r = i / (HD / 4), ch = i % (HD / 4);
+                put_part4(slot + i * 4, *reinterpret_cast<const f4_t*>(om + r * HD + ((ch ^ (r & 7)) << 2)));
+            }
+            if (hh == 0 && w0 + c < w1) put_part(it.slot + it.slot_rows * HD + 2 * (wave * 32 + c), m, l);
+            return;
+        }
         if (w0 + c >= w1) return;
         const int row = wave * 32 + c;
-        float* slot = it.n_parts > 1 ? it.slot : nullptr;
-        if (slot && hh == 0) put_part(slot + it.slot_rows * HD + 2 * row, m, l);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f4_t v = {o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
-                const int at = 32 * d + 8 * q + 4 * hh;
-                if (slot) {
-                    put_part(slot + row * HD + at, v[0], v[1]);
-                    put_part(slot + row * HD + at + 2, v[2], v[3]);
-                } else put_row<T, HD>(L, it, row, at, v, l);
-            }
+            for (int q = 0; q < 4; ++q)
+                put_row<T, HD>(L, it, row, 32 * d + 8 * q + 4 * hh, f4_t{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]}, l);
     }
 };
 
