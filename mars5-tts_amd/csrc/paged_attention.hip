@@ -11,7 +11,7 @@
 //         3 requests of 60 to 120 thousand keys 160 us, 5.5 TB/s; 64 requests with drafts over 1 to 16 thousand keys 309 us, 5.0 TB/s.
 //   many  32x32 matrix instructions.  Each wave owns 32 rows; the waves share 64-key tiles, one barrier per tile.  Bound by the issue of
 //         matrix and vector instructions together (46 % of the cycles matrix, the softmax most of the rest): 2 chunks of 4096 tokens with
-//         contexts of 9 to 12 thousand keys 1580 to 1740 us, 910 to 1000 TFLOP/s.
+//         contexts of 9 to 12 thousand keys 1580 to 1790 us, 880 to 1000 TFLOP/s.
 // K and V rows go from memory into LDS by DMA (global_load_lds, 16 bytes per lane; the page lookup is in the lane's address).  16-byte
 // chunks of a row are stored XOR-swizzled so that the fragment reads spread over all banks (no conflicts counted): K fragments are ds_read_b128, V fragments
 // (keys along the register, features along the lanes) are ds_read_b64_tr_b16, which transposes 4 x 16 blocks on the way, so the
