@@ -38,7 +38,7 @@ M5_HD M5Request m5_request(int start, int end, int seq_len, int n_rows, int64_t 
 
 // Keys that the query at position `pos` of a request with `len` cached positions sees: [lo, hi), empty when lo >= hi.
 M5_HD int m5_key_hi(int pos, int len) { return pos + 1 < len ? pos + 1 : len; }
-M5_HD int m5_key_lo(int pos, int window) { return (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0; }
+M5_HD int m5_key_lo(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }      // (pos may be negative, window 2^31 - 1)
 
 // paged_plan, one request: pages held before, pages needed after; false when the request is not a valid one.
 M5_HD bool m5_plan_request(int held, int keep, int add, int width, int shift, int& have, int& need) {

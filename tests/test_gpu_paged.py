@@ -528,6 +528,32 @@ def test_attention_window(dev, dt, window):
 
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("hd", [64, 128])
+def test_attention_window_wider_than_any_request(dev, dt, hd):
+    """The largest windows give the bits of window 0, also for requests of fewer positions than new rows (the first rows see nothing)."""
+    from mars5_tts_amd import ops
+    lens, new = [3, 300, 40], [6, 70, 41]
+    c = Cache(lens, 2, hd, dt, 16, dev, 15)
+    q = torch.randn(sum(new), 4, hd, generator=torch.Generator().manual_seed(2)).to(dt).to(dev)
+    start = [0, 6, 76, 117]
+    outs = []
+    for window in (0, 1 << 30, (1 << 31) - 1):
+        for max_new in (1, 70):
+            out = torch.full((sum(new), 4, hd), 7.0, dtype=dt, device=dev)
+            ops.paged_attention(q, c.kd, c.vd, c.table_d, _i32(lens, dev), _i32(start, dev), out, window=window, max_new=max_new)
+            outs.append(out)
+    torch.cuda.synchronize()
+    for i in range(2, 6):
+        assert torch.equal(outs[i], outs[i % 2]), i
+    for out in outs[:2]:
+        assert bool((out[:3] == 0).all()) and bool((out[3:6] != 0).any())
+        for b, n in enumerate(lens):
+            m = min(new[b], n)
+            o, A, S, count, V = _attn_ref(q[start[b + 1] - m:start[b + 1]].cpu(), c.k[b], c.v[b], m, 0, hd ** -0.5)
+            assert bool(((out[start[b + 1] - m:start[b + 1]].cpu().double() - o).abs() <= _attn_limit(o, A, S, count, V, dt, hd)).all()), b
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("hd", [64, 128])
 def test_attention_long_split(dev, dt, hd):
     """Few rows over a long axis: keys split over many workgroups and joined; a second call on the same workspace, a smaller and an odd-sized one."""
     from mars5_tts_amd import ops

@@ -88,6 +88,25 @@ def test_key_range_of_a_row(host):
                     assert list(range(lo, max(lo, hi))) == want, (ln, new, window, i)
 
 
+@pytest.mark.parametrize("window", [1 << 30, (1 << 31) - 1])
+def test_a_window_wider_than_any_request_hides_nothing(host, window):
+    """The largest windows that can be passed see what window 0 sees, also where the first rows stand before position 0 (fewer cached
+    positions than new rows)."""
+    o, w, a, b = (C.c_int * 6)(), (C.c_int * 6)(), (C.c_int * 4)(), (C.c_int * 4)()
+    for pos in (-(1 << 30), -7, -3, -2, -1, 0, 1, 1000, (1 << 30) - 1):
+        assert host.h_key_lo(pos, window) == 0
+    for ln in (0, 1, 3, 6, 300):
+        for new in (1, 6, 10, 200):
+            for group, few, many in ((1, 16, 0), (3, 32, 128)):
+                host.h_share(0, new, ln, group, few, many, 0, o)
+                host.h_share(0, new, ln, group, few, many, window, w)
+                assert list(o) == list(w), (ln, new)
+                for t in range(o[2]):
+                    first, last = t * o[1] // group, (min((t + 1) * o[1], o[0]) - 1) // group
+                    seen = [host.h_span(s, ln, win, ln - new + first, ln - new + last, 1, 1 << 24, 0, r) for s, win, r in ((o, 0, a), (w, window, b))]
+                    assert seen == [1, 1] and list(a) == list(b), (ln, new, t)
+
+
 def test_bad_pages_are_no_pages(host):
     for n in (1, 5, 1 << 30):
         for i in BIG:
