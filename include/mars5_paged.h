@@ -62,10 +62,11 @@ typedef struct {
 
 /* Attention of every request's new tokens over its paged cache: query row r of request b (rows q_start[b] .. q_start[b + 1])
  * stands at position p = seq_len[b] - (q_start[b + 1] - r) and sees the keys max(0, p - window + 1) .. p (window 0: from 0 on); query head
- * h reads kv head h / (n_heads / n_kv_heads).  Online softmax in fp32, scores never stored.  A row that sees no key gets zeros;
- * keys on a block id out of range are not seen.  Keys past a request's length and pages behind it are never used, whatever they
- * hold; row offsets that do not ascend compute nothing or rows of theirs twice, inside the buffers.  max_new: upper bound of the
- * new tokens of one request (speed only: it selects the tiling).
+ * h reads kv head h / (n_heads / n_kv_heads).  Online softmax in fp32, scores never stored.  A row that sees no key, or only keys whose
+ * score is -inf, gets zeros; a NaN among the scores that a row sees makes the row NaN; keys on a block id out of range are not seen.
+ * Keys past a request's length and pages behind it are never used, whatever they hold; row offsets that do not ascend compute
+ * nothing or rows of theirs twice, inside the buffers.  max_new: upper bound of the new tokens of one request (speed only: it
+ * selects the tiling).
  * workspace (may be NULL): scratch for keys split over workgroups when there are few rows; zero-filled once by the caller, left
  * ready for the next call of any types and shapes that is given the same bytes; calls that may run at the same time need one
  * each; no other operator's; 16-byte aligned.  More bytes allow more splits; m5_paged_attention_workspace tells how many bytes

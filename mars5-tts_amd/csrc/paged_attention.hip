@@ -825,11 +825,11 @@ __device__ void join_all(const Launch& L, const Item& it, unsigned char* lds) {
                 sum[i] *= alpha;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const float f = k0 + u * groups < it.n_parts ? __builtin_amdgcn_exp2f(ml[i][u].x - use) : 0.f;
-                    if (f != 0.f) {                          // (a part without weight adds nothing, whatever it holds)
-                        l[i] += ml[i][u].y * f;
-                        sum[i] += v[i][u] * f;
-                    }
+                    if (k0 + u * groups >= it.n_parts) continue;     // (the last part, read again)
+                    // a part whose scores are all NaN has m = -inf, so weight 0, and l = NaN, which stays: no part is left out for its weight
+                    const float f = __builtin_amdgcn_exp2f(ml[i][u].x - use);
+                    l[i] += ml[i][u].y * f;
+                    sum[i] += v[i][u] * f;
                 }
             }
         }
@@ -846,10 +846,8 @@ __device__ void join_all(const Launch& L, const Item& it, unsigned char* lds) {
                 for (int g = 1; g < groups; ++g) {
                     const float2 o = meet_ml[g * chunks + at[0]];
                     const float f = __builtin_amdgcn_exp2f(o.x - use);
-                    if (f != 0.f) {
-                        l[0] += o.y * f;
-                        sum[0] += meet[g * chunks + at[0]] * f;
-                    }
+                    l[0] += o.y * f;
+                    sum[0] += meet[g * chunks + at[0]] * f;
                 }
                 m[0] = mn;
             }

@@ -646,6 +646,69 @@ def test_attention_masked_places_do_not_leak(dev, dt, value):
                 assert bool(((got[i] - o[i]).abs() <= lim[i]).all()), (heads, hd, i)
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [[1, 2], [5, 1], [90, 1]])
+def test_attention_nan_that_a_row_sees(dev, dt, hd, new):
+    """A NaN in a query's row, or in all keys of one kv head over a range as long as a chunk: exactly those heads of the rows that see it come out as
+    NaN, whether their keys are split over workgroups or not; all others as if it were not there."""
+    from mars5_tts_amd import ops
+    heads, kv, ctx, far = 4, 2, [3000, 1500], 2000
+    lens, rows = [a + b for a, b in zip(ctx, new)], sum(new)
+    start = [0, new[0], rows]
+    for where in ("query", "keys"):
+        c = Cache(lens, kv, hd, dt, 16, dev, 17)
+        q = torch.randn(rows, heads, hd, generator=torch.Generator().manual_seed(3)).to(dt)
+        poisoned = torch.zeros(rows, heads, dtype=torch.bool)
+        qd = q.to(dev)
+        if where == "query":
+            qd[new[0] - 1, 1, 5] = float("nan")
+            qd[rows - 1, 2, 0] = float("nan")
+            poisoned[new[0] - 1, 1] = poisoned[rows - 1, 2] = True
+        else:
+            c.kd[c.table[0, :far // 16].long().to(dev), 1] = float("nan")        # request 0, its first 2000 keys, kv head 1
+            poisoned[:new[0], 2:] = True
+        for ws in (None, torch.zeros(24 << 20, dtype=torch.uint8, device=dev), torch.zeros(1 << 20, dtype=torch.uint8, device=dev)):
+            out = torch.full((rows, heads, hd), 7.0, dtype=dt, device=dev)
+            ops.paged_attention(qd, c.kd, c.vd, c.table_d, _i32(lens, dev), _i32(start, dev), out, max_new=max(new), workspace=ws)
+            torch.cuda.synchronize()
+            got = out.cpu().double()
+            assert bool(torch.isnan(got[poisoned]).all()), (where, "a NaN was lost")
+            for b in range(2):
+                lo, hi = start[b], start[b + 1]
+                o, A, S, count, V = _attn_ref(q[lo:hi], c.k[b], c.v[b], new[b], 0, hd ** -0.5)
+                fine = (got[lo:hi] - o).abs() <= _attn_limit(o, A, S, count, V, dt, hd)
+                assert bool((fine | poisoned[lo:hi, :, None]).all()), (where, b)
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [[1, 2], [90, 1]])
+def test_attention_scores_of_minus_infinity(dev, dt, hd, new):
+    """Keys whose score is -inf have no weight; a row all of whose scores are -inf gets zeros, as one that sees no key; split and not."""
+    from mars5_tts_amd import ops
+    heads, kv, ctx = 4, 2, [3000, 700]
+    lens, rows = [a + b for a, b in zip(ctx, new)], sum(new)
+    start = [0, new[0], rows]
+    c = Cache(lens, kv, hd, dt, 16, dev, 18)
+    q = torch.randn(rows, heads, hd, generator=torch.Generator().manual_seed(4)).to(dt)
+    q[..., 0] = 1.0                                                              # so a key of -inf in feature 0 scores -inf
+    hide = torch.zeros(lens[0], dtype=torch.bool)
+    hide[512:1900] = True                                                        # request 0: whole chunks of its keys and parts of others
+    hide[2999] = True
+    for p in hide.nonzero()[:, 0].tolist():
+        c.kd[int(c.table[0, p // 16]), :, p % 16, 0] = -float("inf")
+    c.kd[c.table[1, :-(-lens[1] // 16)].long().to(dev), :, :, 0] = -float("inf")     # request 1: all of them
+    for ws in (None, torch.zeros(24 << 20, dtype=torch.uint8, device=dev)):
+        out = torch.full((rows, heads, hd), 7.0, dtype=dt, device=dev)
+        ops.paged_attention(q.to(dev), c.kd, c.vd, c.table_d, _i32(lens, dev), _i32(start, dev), out, max_new=max(new), workspace=ws)
+        torch.cuda.synchronize()
+        got = out.cpu().double()
+        o, A, S, count, V = _attn_ref(q[:new[0]], c.k[0], c.v[0], new[0], 0, hd ** -0.5, hide)
+        assert bool(((got[:new[0]] - o).abs() <= _attn_limit(o, A, S, count, V, dt, hd)).all())
+        assert bool((got[new[0]:] == 0).all())
+
+
 def test_attention_offsets_past_32_bits(dev):
     """Block strides so far apart that byte and element offsets pass 2^31: two blocks at the ends of a cache of 2.3e9 elements."""
     from mars5_tts_amd import ops
