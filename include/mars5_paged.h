@@ -95,6 +95,9 @@ typedef struct {
  *   out_tokens[b] = accepted drafts, the drawn token, then -1;  n_out[b] = their number (0 for a request without rows)
  *   keep_len[b] = seq_len[b] - (r1 - r0) + n_out[b] (both NULL: not wanted): positions that m5_paged_plan keeps in the next step
  * dtype: that of target and draft.  A request of more than out_width rows counts its first out_width rows.
+ * plan_state (may be NULL): the state of the m5_paged_plan that opened the step.  If that refused the step (status not 0), every
+ * request counts as one without rows and keep_len is left as it was: seq_len still holds what the step before rejected, so a keep_len
+ * given to the plan must outlive it, and the step can be tried again once there are blocks.
  * workspace (may be NULL): M5_DRAFT_WS_BYTES per request, kept as m5_paged_attention's; lets a row be split over workgroups. */
 #define M5_DRAFT_WS_BYTES 32
 typedef struct {
@@ -106,6 +109,7 @@ typedef struct {
     int64_t* out_tokens; int64_t out_rs; int32_t* n_out;
     const int32_t* seq_len; int32_t* keep_len;
     void* workspace; int64_t workspace_bytes;
+    const int32_t* plan_state;
 } M5DraftVerifyArgs;
 
 #endif /* MARS5_PAGED_H */

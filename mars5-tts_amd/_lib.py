@@ -183,7 +183,7 @@ class DraftVerifyArgs(C.Structure):
                 ("n_rows", i32), ("vocab", i32), ("n_seq", i32), ("out_width", i32),
                 ("tokens", vp), ("row_start", vp), ("uniforms", vp), ("noise", vp), ("noise_rs", i64),
                 ("out_tokens", vp), ("out_rs", i64), ("n_out", vp), ("seq_len", vp), ("keep_len", vp),
-                ("workspace", vp), ("workspace_bytes", i64)]
+                ("workspace", vp), ("workspace_bytes", i64), ("plan_state", vp)]
 
 
 def packed(cls):

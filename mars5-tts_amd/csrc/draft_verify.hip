@@ -45,8 +45,9 @@ __global__ __launch_bounds__(NT) void draft_verify_kernel(M5DraftVerifyArgs p, i
     __shared__ unsigned long long wk[2][NT / 64];
     __shared__ int sh_count, sh_any[NT / 64], sh_last;
     const int b = blockIdx.x / parts, part = blockIdx.x % parts, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const bool refused = p.plan_state && p.plan_state[M5_PST_STATUS] != 0;       // no rows, and keep_len stays the plan's
     const M5Request rq = m5_request(p.row_start[b], p.row_start[b + 1], 0, p.n_rows, 0);
-    const int rows = rq.r1 - rq.r0, n = min(rows, p.out_width);
+    const int rows = refused ? 0 : rq.r1 - rq.r0, n = min(rows, p.out_width);
     const st* target = (const st*)p.target;
     const st* draft = (const st*)p.draft;
     if (wave == 0) {                                         // drafts accepted before the first that is not
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(NT) void draft_verify_kernel(M5DraftVerifyArgs p, i
             const unsigned long long key = some ? best : plain;
             wk[0][0] = key ? (uint32_t)~(uint32_t)key : 0u;
             p.n_out[b] = n > 0 ? count + 1 : 0;
-            if (p.keep_len) p.keep_len[b] = p.seq_len[b] - rows + (n > 0 ? count + 1 : 0);
+            if (p.keep_len && !refused) p.keep_len[b] = p.seq_len[b] - rows + (n > 0 ? count + 1 : 0);
         }
         sh_last = last;
     }

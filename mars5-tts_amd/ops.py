@@ -426,12 +426,14 @@ def paged_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
 
 def draft_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor, row_start: torch.Tensor, uniforms: torch.Tensor,
                  noise: torch.Tensor, out_tokens: torch.Tensor, n_out: torch.Tensor, seq_len: Optional[torch.Tensor] = None,
-                 keep_len: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
+                 keep_len: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream: Optional[int] = None,
+                 plan_state: Optional[torch.Tensor] = None) -> None:
     """Speculative sampling from given random numbers: target / draft (n_rows, vocab) probabilities (draft None: certain drafts),
     tokens (n_rows,) int64 the tokens that were fed, row_start (n_seq + 1,) int32, uniforms (n_rows,) and noise (n_seq, vocab)
     fp32 (U[0, 1) and Exp(1)).  out_tokens (n_seq, width) int64 = accepted drafts, one drawn token, -1; n_out (n_seq,) int32;
     keep_len = seq_len - rows + n_out for the next paged_plan.  workspace: DRAFT_WS_BYTES per request (uint8, zero-filled once, one
-    for every call that may be in flight at a time), or None.  One launch."""
+    for every call that may be in flight at a time), or None.  plan_state: the state of the step's paged_plan; if that refused the
+    step, nothing is verified and keep_len (the tensor that the plan was given) stays as it was.  One launch."""
     idx, (rows, V), (B,), dt = target.get_device(), target.shape, n_out.shape, target.dtype
     assert idx >= 0, _NO_DEVICE
     assert (idx == tokens.get_device() == row_start.get_device() == uniforms.get_device() == noise.get_device() == out_tokens.get_device() ==
@@ -443,7 +445,7 @@ def draft_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: to
     assert out_tokens.dtype == _I64 and out_tokens.dim() == 2 and out_tokens.shape[0] == B and out_tokens.stride(1) == 1, "out_tokens: (n_seq, width) int64"
     assert row_start.dtype == n_out.dtype == _I32 and row_start.shape == (B + 1,) and row_start.is_contiguous() and n_out.is_contiguous(), "row_start (n_seq + 1,), n_out (n_seq,): int32"
     assert (seq_len is None) == (keep_len is None), "seq_len and keep_len go together"
-    q = q_rs = held = kept = ws = ws_bytes = 0
+    q = q_rs = held = kept = ws = ws_bytes = words = 0
     if draft is not None:
         assert draft.shape == target.shape and draft.dtype == dt and draft.stride(1) == 1 and draft.get_device() == idx, "draft: target's shape and type"
         q, q_rs = draft.data_ptr(), draft.stride(0)
@@ -454,8 +456,11 @@ def draft_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: to
     if workspace is not None:
         assert workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous() and workspace.get_device() == idx, "workspace: zero-filled uint8 bytes"
         ws, ws_bytes = workspace.data_ptr(), workspace.shape[0]
+    if plan_state is not None:
+        assert plan_state.dtype == _I32 and plan_state.shape == (L.PST_WORDS,) and plan_state.is_contiguous() and plan_state.get_device() == idx, "plan_state: (PST_WORDS,) int32"
+        words = plan_state.data_ptr()
     args = _verify_args(target.data_ptr(), target.stride(0), q, q_rs, rows, V, B, out_tokens.shape[1], tokens.data_ptr(), row_start.data_ptr(), uniforms.data_ptr(),
-                        noise.data_ptr(), noise.stride(0), out_tokens.data_ptr(), out_tokens.stride(0), n_out.data_ptr(), held, kept, ws, ws_bytes)
+                        noise.data_ptr(), noise.stride(0), out_tokens.data_ptr(), out_tokens.stride(0), n_out.data_ptr(), held, kept, ws, ws_bytes, words)
     _launch(_verify, "m5_draft_verify", (DT_CODE[dt],), C.byref(args), idx, stream)
 
 

@@ -1052,6 +1052,60 @@ def test_speculative_serving_run(dev):
     assert sorted(t["free"].tolist()) == list(range(n_blocks)) and int(t["state"][L.PST_FREE]) == n_blocks
 
 
+@pytest.mark.parametrize("V", [50, 9000])
+@pytest.mark.parametrize("recorded", [False, True])
+def test_refused_step_keeps_the_pending_roll_back(dev, recorded, V):
+    """Drafts are rejected, the next step is short of blocks (or holds an invalid request), verification runs behind it as in every step: keep_len
+    stays what the plan was given, so the step that is tried again once a request has ended gives back the rejected positions.  As
+    calls and as a recorded plan; the list definition throughout."""
+    from mars5_tts_amd import _lib as L, ops
+    B, block, width, n_blocks, M, rows = 3, 4, 8, 7, 5, 40
+    pool = Pool(B, width, n_blocks, block, 4)
+    t = pool.tensors(dev)
+    keep, new = _i32([0] * B, dev), _i32([0] * B, dev)
+    q_start, slots, pos = _i32([7] * (B + 1), dev), _i32([7] * rows, dev), _i32([7] * rows, dev)
+    g = torch.Generator().manual_seed(6)
+    target = torch.softmax(torch.randn(rows, V, generator=g), -1)
+    draft = torch.softmax(torch.randn(rows, V, generator=g), -1)
+    tokens, uni, noise = torch.randint(0, V, (rows,), generator=g), torch.ones(rows), torch.empty(B, V).exponential_(generator=g)
+    dense = [x.to(dev) for x in (target, draft, tokens, uni, noise)]
+    out, n_out = torch.zeros(B, M, dtype=torch.int64, device=dev), _i32([0] * B, dev)
+    vs = torch.zeros(B * L.DRAFT_WS_BYTES, dtype=torch.uint8, device=dev)
+
+    def calls():
+        ops.paged_plan(t["seq_len"], keep, new, t["table"], t["free"], t["state"], block, q_start, slots, pos)
+        ops.draft_verify(dense[0], dense[1], dense[2], q_start, dense[3], dense[4], out, n_out, seq_len=t["seq_len"], keep_len=keep, workspace=vs, plan_state=t["state"])
+
+    plan = None
+    if recorded:
+        plan = ops.StagePlan("ar_decode_step")
+        with plan.recording():
+            calls()
+    kept, statuses = [0] * B, []
+    # (what the host wants added, requests that it ends before): the third and fourth step cannot be served
+    for add, ended in (([3, 5, 2], []), ([5, 4, 4], []), ([8, 8, 8], []), ([4, 1, width * block], []), ([2, 0, 5], [1]), ([1, 3, 0], [])):
+        for b in ended:
+            kept[b] = 0
+            keep[b] = 0
+        new.copy_(_i32(add, dev))
+        assert keep.tolist() == kept
+        want = pool.step(kept[:], add, rows)
+        plan.run() if recorded else calls()
+        torch.cuda.synchronize()
+        _check_plan(t, pool, want, q_start, slots, pos)
+        w_out, w_n, w_keep = _verify_ref(target, draft, tokens, want[1], uni, noise, M, pool.len)
+        assert out.tolist() == w_out and n_out.tolist() == w_n
+        if want[0] == 0:
+            kept = w_keep
+        assert keep.tolist() == kept, want[0]
+        statuses.append(want[0])
+    assert not bool(vs.any())                                                    # (the larger vocabulary is split: its workgroups have met)
+    assert statuses[2] > 0 and statuses[3] < 0 and [s for i, s in enumerate(statuses) if i not in (2, 3)] == [0] * 4
+    for bad in (t["state"][:4], t["state"].long(), t["state"].cpu()):
+        with pytest.raises(AssertionError, match="plan_state"):
+            ops.draft_verify(dense[0], dense[1], dense[2], q_start, dense[3], dense[4], out, n_out, plan_state=bad)
+
+
 def test_recorded_step_equals_the_calls(dev):
     """A whole step recorded as a stage plan: run from C, then captured into a graph and replayed, beside the same calls one by one; the
     keep_len that verification writes is the next step's, so every step depends on the ones before."""
