@@ -629,7 +629,6 @@ struct Many {
                 const unsigned char* ks = lds + stage * STAGE_B;
                 const unsigned char* vs = ks + OP_B;
                 const bool whole = there == ~0ull && kb + KT - 1 <= pos_min && kb >= lo_max;
-                unsigned long long vis = 0;
                 f16_t s[2];
                 uint4 kf[2][NF];
 #pragma unroll
@@ -656,7 +655,7 @@ struct Many {
                 }
                 __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, NF, 0);
                 if (!whole) {
-                    vis = seen(there, kb, lo, qpos);
+                    const unsigned long long vis = seen(there, kb, lo, qpos);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t half = (uint32_t)(vis >> (32 * h + 4 * hh));
@@ -720,7 +719,8 @@ struct Many {
                     __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, ND, 1);
                 }
                 __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, ND, 1);
-                if (odd) {
+                if (odd) {                                       // (of the workgroup: this wave's rows may see the tile whole)
+                    const unsigned long long vis = seen(there, kb, lo, qpos);
                     int at = 4 * hh;
                     asm volatile("" : "+v"(at));                 // (computed here: the compiler would keep an address per feature in registers)
 #pragma unroll

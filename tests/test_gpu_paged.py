@@ -709,6 +709,44 @@ def test_attention_scores_of_minus_infinity(dev, dt, hd, new):
         assert bool((got[new[0]:] == 0).all())
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("heads,kv,hd,new,n,window", [(4, 2, 64, 70, 130, 0), (4, 4, 128, 9, 90, 0), (2, 1, 128, 75, 300, 50), (8, 1, 64, 2, 64, 0), (6, 2, 64, 5, 2500, 0),
+                                                      (4, 2, 128, 60, 3000, 0), (1, 1, 64, 1, 5, 0), (4, 1, 128, 4, 1100, 700)])
+def test_attention_nonfinite_values_reach_the_rows_that_see_them(dev, dt, heads, kv, hd, new, n, window, split):
+    """Infinite and NaN features of VALUES alone: exactly the rows that see the key get +inf, -inf or NaN (both signs: NaN), at exactly those
+    features of the kv head's query heads; every other feature and row comes out as if they were finite."""
+    from mars5_tts_amd import ops
+    inf, nan = float("inf"), float("nan")
+    c = Cache([n], kv, hd, dt, 16, dev, 19)
+    q = torch.randn(new, heads, hd, generator=torch.Generator().manual_seed(5)).to(dt)
+    at = n - 1 - new // 2                                            # seen by the later half of the rows
+    spots = [(at, 0, 3, inf), (at, kv - 1, hd - 1, -inf), (min(at + 1, n - 1), 0, 3, -inf), (at, 0, 17, nan), (n - 1, kv - 1, 40, inf), (0, kv - 1, 41, inf),
+             (max(n - new - 40, 0), 0, 8, -inf), (max(n - new - 41, 0), 0, 9, nan), (n // 2, 0, 10, inf), (n // 2, 0, 11, -inf)]
+    rep = heads // kv
+    plus, minus = (torch.zeros(new, heads, hd, dtype=torch.bool) for _ in range(2))
+    for (p, h, d), value in {spot[:3]: spot[3] for spot in spots}.items():       # (one value a place: the last)
+        c.vd[int(c.table[0, p // 16]), h, p % 16, d] = value
+        for i in range(new):
+            pos = n - new + i
+            if p <= pos and (not window or p > pos - window):
+                if not value < 0:
+                    plus[i, h * rep:(h + 1) * rep, d] = True
+                if not value > 0:
+                    minus[i, h * rep:(h + 1) * rep, d] = True
+    ws = torch.zeros(24 << 20, dtype=torch.uint8, device=dev) if split else None
+    o, A, S, count, V = _attn_ref(q, c.k[0], c.v[0], new, window, hd ** -0.5)
+    lim = _attn_limit(o, A, S, count, V, dt, hd)
+    for max_new in (new, 1):                                         # (large and small tiles)
+        out = torch.full((new, heads, hd), 7.0, dtype=dt, device=dev)
+        ops.paged_attention(q.to(dev), c.kd, c.vd, c.table_d, _i32([n], dev), _i32([0, new], dev), out, window=window, max_new=max_new, workspace=ws)
+        torch.cuda.synchronize()
+        got = out.cpu().double()
+        assert bool((got[plus & ~minus] == inf).all()) and bool((got[minus & ~plus] == -inf).all()) and bool(torch.isnan(got[plus & minus]).all())
+        finite = ~(plus | minus)
+        assert bool(((got - o).abs() <= lim)[finite].all())
+
+
 def test_attention_offsets_past_32_bits(dev):
     """Block strides so far apart that byte and element offsets pass 2^31: two blocks at the ends of a cache of 2.3e9 elements."""
     from mars5_tts_amd import ops
