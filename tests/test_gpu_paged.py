@@ -747,6 +747,44 @@ def test_attention_nonfinite_values_reach_the_rows_that_see_them(dev, dt, heads,
         assert bool(((got - o).abs() <= lim)[finite].all())
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ctx", [40, 3000])
+def test_attention_row_offsets_claimed_twice(dev, dt, hd, ctx):
+    """Row offsets that do not ascend, over a buffer with guards: requests that claim the same rows compute nothing or those rows (they hold the same
+    positions here, so the result is theirs); nothing outside the claimed rows is written, with and without
+    room to split, and the workspace is left ready."""
+    from mars5_tts_amd import ops
+    rows, heads, kv = 100, 4, 2
+    c = Cache([ctx + rows], kv, hd, dt, 16, dev, 23)
+    q = torch.randn(rows, heads, hd, generator=torch.Generator().manual_seed(6)).to(dt)
+    o, A, S, count, V = _attn_ref(q, c.k[0], c.v[0], rows, 0, hd ** -0.5)
+    lim = _attn_limit(o, A, S, count, V, dt, hd)
+    qd = torch.zeros(rows + 64, heads, hd, dtype=dt, device=dev)
+    qd[:rows] = q.to(dev)
+    for B in (5, 201):
+        table = c.table.expand(B, -1).contiguous().to(dev)
+        start = [0 if b % 2 == 0 else rows for b in range(B + 1)]            # 0 .. rows, rows .. 0, 0 .. rows, ...
+        for max_new in (1, rows):
+            for ws in (None, torch.zeros(24 << 20, dtype=torch.uint8, device=dev), torch.zeros(200000, dtype=torch.uint8, device=dev)):
+                buf = torch.full((rows + 128, heads, hd), 7.0, dtype=dt, device=dev)
+                out = buf[32:32 + rows + 64]
+                ops.paged_attention(qd, c.kd, c.vd, table, _i32([ctx + rows] * B, dev), _i32(start, dev), out, max_new=max_new, workspace=ws)
+                torch.cuda.synchronize()
+                assert bool((buf[:32] == 7.0).all()) and bool((buf[32 + rows:] == 7.0).all())
+                got = out[:rows].cpu().double()
+                nothing = bool((got == 7.0).all())
+                assert nothing or bool(((got - o).abs() <= lim).all())
+                if max_new == 1:
+                    assert nothing                                           # more small tiles than the rows can make
+                elif B == 5 and dt != torch.float32:
+                    assert not nothing                                       # few enough large ones to pass for valid
+                if ws is not None:
+                    ops.paged_attention(qd[:rows], c.kd, c.vd, table[:1], _i32([ctx + rows], dev), _i32([0, rows], dev), out[:rows], max_new=max_new, workspace=ws)
+                    torch.cuda.synchronize()
+                    assert bool(((out[:rows].cpu().double() - o).abs() <= lim).all()) and not bool(ws[:160].any())
+
+
 def test_attention_offsets_past_32_bits(dev):
     """Block strides so far apart that byte and element offsets pass 2^31: two blocks at the ends of a cache of 2.3e9 elements."""
     from mars5_tts_amd import ops
