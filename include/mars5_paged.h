@@ -94,6 +94,9 @@ typedef struct {
  * (noise: Exp(1) draws as in m5_ar_sample; NaN and weights <= 0 count as 0).
  *   out_tokens[b] = accepted drafts, the drawn token, then -1;  n_out[b] = their number (0 for a request without rows)
  *   keep_len[b] = seq_len[b] - (r1 - r0) + n_out[b] (both NULL: not wanted): positions that m5_paged_plan keeps in the next step
+ * row_start is the plan's q_start only where a request's rows are one sampled token and the drafts behind it: a prompt's rows would be taken
+ * for drafts.  Of a prompt's chunk only the last row is verified (none while more of the prompt is to come): rows and offsets of
+ * their own; keep_len then keeps the chunk whole.
  * dtype: that of target and draft.  A request of more than out_width rows counts its first out_width rows.
  * plan_state (may be NULL): the state of the m5_paged_plan that opened the step.  If that refused the step (status not 0), every
  * request counts as one without rows and keep_len is left as it was: seq_len still holds what the step before rejected, so a keep_len

@@ -433,7 +433,8 @@ def draft_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: to
     fp32 (U[0, 1) and Exp(1)).  out_tokens (n_seq, width) int64 = accepted drafts, one drawn token, -1; n_out (n_seq,) int32;
     keep_len = seq_len - rows + n_out for the next paged_plan.  workspace: DRAFT_WS_BYTES per request (uint8, zero-filled once, one
     for every call that may be in flight at a time), or None.  plan_state: the state of the step's paged_plan; if that refused the
-    step, nothing is verified and keep_len (the tensor that the plan was given) stays as it was.  One launch."""
+    step, nothing is verified and keep_len (the tensor that the plan was given) stays as it was.  row_start is the plan's q_start only in
+    steps without prompt chunks: of those, the last row alone is verified (include/mars5_paged.h).  One launch."""
     idx, (rows, V), (B,), dt = target.get_device(), target.shape, n_out.shape, target.dtype
     assert idx >= 0, _NO_DEVICE
     assert (idx == tokens.get_device() == row_start.get_device() == uniforms.get_device() == noise.get_device() == out_tokens.get_device() ==

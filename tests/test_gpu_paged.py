@@ -1128,6 +1128,83 @@ def test_speculative_serving_run(dev):
     assert sorted(t["free"].tolist()) == list(range(n_blocks)) and int(t["state"][L.PST_FREE]) == n_blocks
 
 
+def _rows_to_verify(q_start, n_verify, cap, n_rows):
+    """The last n_verify[b] rows of every request, packed (cap rows, the last ones padding), and their row offsets: device work only.  Requests
+    without rows in this step (or a refused one) verify nothing."""
+    n = torch.minimum(n_verify, q_start[1:] - q_start[:-1])
+    row_start = torch.zeros_like(q_start)
+    row_start[1:] = torch.cumsum(n, 0)
+    i = torch.arange(cap, dtype=torch.int32, device=q_start.device)
+    b = torch.searchsorted(row_start[1:], i, right=True).clamp(max=n.shape[0] - 1)
+    return (q_start[b + 1] - row_start[b + 1] + i).clamp(0, n_rows - 1), row_start
+
+
+def test_steps_of_prompt_chunks_and_drafts(dev):
+    """Prompts that arrive in chunks beside requests that draft: only a prompt's last row is verified (a chunk that is not the last: none), so every
+    prompt stays whole in the cache; rows, row offsets and kept lengths are found on the device, without a read-back inside the step.  Probabilities
+    against a cache-free float64 recomputation, tokens and kept lengths against the definition."""
+    from mars5_tts_amd import _lib as L, ops
+    lm = _TinyLM(dev, seed=3).to(dev)
+    B, block, width, n_blocks, K, V, chunk, rows, cap = 4, 8, 12, 40, 4, lm.vocab, 10, 36, 18
+    g = torch.Generator().manual_seed(15)
+    pool = Pool(B, width, n_blocks, block, 2)
+    t = pool.tensors(dev)
+    caches = [tuple(torch.full((n_blocks, lm.kv, block, lm.hd), float("nan"), device=dev) for _ in range(2)) for _ in range(2)]
+    ws = torch.zeros(4 << 20, dtype=torch.uint8, device=dev)
+    vs = torch.zeros(B * L.DRAFT_WS_BYTES, dtype=torch.uint8, device=dev)
+    prompts = [torch.randint(0, V, (n,), generator=g).tolist() for n in (23, 1, 10, 30)]
+    seqs = [[] for _ in range(B)]                                                # ids in the cache
+    keep, out, n_out = _i32([0] * B, dev), torch.zeros(B, K + 1, dtype=torch.int64, device=dev), _i32([0] * B, dev)
+    drawn = [None] * B
+    q_start, slots, pos = _i32([0] * (B + 1), dev), _i32([0] * rows, dev), _i32([0] * rows, dev)
+    mixed = 0
+    for step in range(7):
+        feed, verify = [], []
+        for b in range(B):
+            if prompts[b]:
+                feed.append(prompts[b][:chunk])
+                prompts[b] = prompts[b][chunk:]
+                verify.append(0 if prompts[b] else 1)
+            else:
+                feed.append([drawn[b]] + torch.randint(0, V, ((step * 3 + b) % K,), generator=g).tolist())
+                verify.append(len(feed[b]))
+            seqs[b] = seqs[b] + feed[b]
+        new = [len(f) for f in feed]
+        flat = [i for f in feed for i in f]
+        mixed += max(new) == chunk and any(v > 1 for v in verify)
+        ids = torch.tensor(flat + [0] * (rows - len(flat)), device=dev)
+        uni, noise = torch.rand(cap, generator=g), torch.empty(B, V).exponential_(generator=g)
+        args = [_i32(new, dev), _i32(verify, dev), uni.to(dev), noise.to(dev)]
+        # ---- the step: nothing is read back
+        ops.paged_plan(t["seq_len"], keep, args[0], t["table"], t["free"], t["state"], block, q_start, slots, pos)
+        probs = lm.forward(ids, pos, slots, caches, t["table"], t["seq_len"], q_start, rows, chunk, ws)
+        sel, row_start = _rows_to_verify(q_start, args[1], cap, rows)
+        target = probs[sel]
+        draft = torch.full((cap, V), 1.0 / V, device=dev)
+        ops.draft_verify(target, draft, ids[sel], row_start, args[2], args[3], out, n_out, seq_len=t["seq_len"], keep_len=keep, workspace=vs, plan_state=t["state"])
+        # ---- checks
+        assert int(t["state"][L.PST_STATUS]) == 0
+        start = [0]
+        for n in new:
+            start.append(start[-1] + n)
+        rs = [0]
+        for n in verify:
+            rs.append(rs[-1] + n)
+        assert row_start.tolist() == rs and sel[:rs[-1]].tolist() == [r for b in range(B) for r in range(start[b + 1] - verify[b], start[b + 1])]
+        for b in range(B):
+            want = lm.reference(seqs[b])[-new[b]:]
+            # (as above: two layers of fp32 products of 256 terms)
+            assert float((probs[start[b]:start[b + 1]].cpu().double() - want).abs().max()) < 1e-4, (step, b)
+        w_out, w_n, w_keep = _verify_ref(target.cpu(), draft.cpu(), ids[sel].cpu(), rs, uni, noise, K + 1, [len(q) for q in seqs])
+        assert out.tolist() == w_out and n_out.tolist() == w_n and keep.tolist() == w_keep
+        for b in range(B):
+            if prompts[b] or verify[b] == 1:
+                assert w_keep[b] == len(seqs[b])                                 # a prompt (or a lone token) stays whole
+            seqs[b] = seqs[b][:w_keep[b]]
+            drawn[b] = w_out[b][w_n[b] - 1] if w_n[b] else None
+    assert mixed >= 2
+
+
 @pytest.mark.parametrize("V", [50, 9000])
 @pytest.mark.parametrize("recorded", [False, True])
 def test_refused_step_keeps_the_pending_roll_back(dev, recorded, V):
