@@ -209,13 +209,18 @@ __device__ inline float2 get_part(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-// softmax state of one row block: new maximum from this lane's scores (already reduced over the lanes of the row)
+// p = exp2(s sc2 - use), use = m sc2 rounded, in one fused operation.  Its residue, up to half a unit of the last place of use, is the same factor
+// for all that a row adds up and cancels, but from 2^24 on the unit is 2 and more and p may leave the operand type (fp16 first) or 32 bits: there
+// exp2((s - m) sc2) is taken, whose difference is exact for the scores that count.
+constexpr float FAR_SCORE = 1 << 24;
+
+// softmax state of one row block: new maximum from this lane's scores (already reduced over the lanes of the row); m: of the scores unscaled
 struct Soft {
     float m, l;
-    __device__ inline float step(float mx, float& use) {     // returns the factor of everything accumulated so far
+    __device__ inline float step(float mx, float sc2, float& use) {       // returns the factor of everything accumulated so far
         const float mn = fmaxf(m, mx);
-        use = mn == -INFINITY ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - use);
+        use = mn == -INFINITY ? 0.f : mn * sc2;
+        const float alpha = __builtin_amdgcn_exp2f(m * sc2 - use);
         m = mn;
         return alpha;
     }
@@ -415,9 +420,15 @@ struct Few {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rb][h][r]);
                     mx = fmaxf(mx, lane_xor16(mx));
-                    mx = fmaxf(mx, lane_xor32(mx)) * L.sc2;
+                    mx = fmaxf(mx, lane_xor32(mx));
                     float use;
-                    const float alpha = sm[rb].step(mx, use);
+                    const float alpha = sm[rb].step(mx, L.sc2, use);
+                    if (__any(fabsf(use) >= FAR_SCORE)) {
+                        const float base = fabsf(use) >= FAR_SCORE ? sm[rb].m : 0.f;
+#pragma unroll
+                        for (int h = 0; h < SUB; ++h) s[rb][h] -= base;
+                        use = base != 0.f ? 0.f : use;
+                    }
                     float sum = 0.f;
                     __attribute__((aligned(16))) st e[4 * SUB];
 #pragma unroll
@@ -480,7 +491,7 @@ struct Few {
             l += lane_xor16(l);
             l += lane_xor32(l);
             const int row = rb * 16 + c;
-            if (g == 0) { ml[(wave * 32 + row) * 2] = sm[rb].m; ml[(wave * 32 + row) * 2 + 1] = l; }
+            if (g == 0) { ml[(wave * 32 + row) * 2] = sm[rb].m * L.sc2; ml[(wave * 32 + row) * 2 + 1] = l; }
 #pragma unroll
             for (int d = 0; d < ND; ++d) *reinterpret_cast<f4_t*>(om + row * HD + (((4 * d + g) ^ (row & 15)) << 2)) = o[rb][d];
         }
@@ -666,17 +677,24 @@ struct Many {
                 float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
                 for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, s[0][r]), s[1][r]);
-                mx = fmaxf(mx, lane_xor32(mx)) * L.sc2;
+                mx = fmaxf(mx, lane_xor32(mx));
                 // p = exp2(s - m) with an m that is raised only when a score passes it by more than 8: p stays below 2^8, which the operand
                 // types hold with the same relative error, and most tiles spare the rescaling of o (64 or 32 products per lane)
-                if (__any(mx > m + 8.f)) {
+                if (__any((mx - m) * L.sc2 > 8.f)) {
                     const float mn = fmaxf(m, mx);
-                    use = mn == -INFINITY ? 0.f : mn;
-                    const float alpha = __builtin_amdgcn_exp2f(m - use);
+                    use = mn == -INFINITY ? 0.f : mn * L.sc2;
+                    const float alpha = __builtin_amdgcn_exp2f(m * L.sc2 - use);
                     m = mn;
                     l *= alpha;
 #pragma unroll
                     for (int d = 0; d < ND; ++d) o[d] *= alpha;
+                }
+                float minus = use;
+                if (__any(fabsf(use) >= FAR_SCORE)) {
+                    const float base = fabsf(use) >= FAR_SCORE ? m : 0.f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) s[h] -= base;
+                    minus = base != 0.f ? 0.f : use;
                 }
                 uint4 pf[2][2];
 #pragma unroll
@@ -687,7 +705,7 @@ struct Many {
                         float x[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][8 * k + j], L.sc2, -use));
+                            x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][8 * k + j], L.sc2, -minus));
                             e[j] = T::from_f32(x[j]);
                         }
                         pf[h][k] = *reinterpret_cast<const uint4*>(e);
@@ -763,7 +781,7 @@ struct Many {
                 const int r = i / (HD / 4), ch = i % (HD / 4);
                 put_part4(slot + i * 4, *reinterpret_cast<const f4_t*>(om + r * HD + ((ch ^ (r & 7)) << 2)));
             }
-            if (hh == 0 && w0 + c < w1) put_part(it.slot + it.slot_rows * HD + 2 * (wave * 32 + c), m, l);
+            if (hh == 0 && w0 + c < w1) put_part(it.slot + it.slot_rows * HD + 2 * (wave * 32 + c), m * L.sc2, l);
             return;
         }
         if (w0 + c >= w1) return;

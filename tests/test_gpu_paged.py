@@ -580,6 +580,38 @@ def test_attention_large_scores_and_scale(dev):
 
 
 @pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** 6, 2.0 ** 10, 2.0 ** 20])
+def test_attention_scores_past_the_exponents_fraction(dev, dt, hd, scale):
+    """Scores up to 1e13, positive and negative, where a unit of the last place of a score is many powers of e: the keys of the largest score share
+    the weight (the scores here are whole numbers times the scale, exact in 32 bits, and differ by 2^15 scale or not at all)."""
+    from mars5_tts_amd import ops
+    heads, kv, ctx, new = 4, 2, [2500, 300, 40], [1, 70, 3]
+    lens, start = [a + b for a, b in zip(ctx, new)], [0, 1, 71, 74]
+    for sign in (1.0, -1.0):
+        c = Cache(lens, kv, hd, dt, 16, dev, 29)
+        q = torch.zeros(74, heads, hd, dtype=dt)
+        q[..., 0] = 32768.0
+        g = torch.Generator().manual_seed(8)
+        for b, n in enumerate(lens):
+            k = torch.zeros(n, kv, hd, dtype=dt)
+            k[..., 0] = sign * torch.randint(1, 200, (n, kv), generator=g).to(dt)
+            c.k[b] = k
+            j = torch.arange(n)
+            c.kd[c.table[b].long()[j // 16].to(dev), :, (j % 16).to(dev)] = k.to(dev)
+        for max_new in (70, 1):
+            for ws in (None, torch.zeros(24 << 20, dtype=torch.uint8, device=dev)):
+                out = torch.full((74, heads, hd), 7.0, dtype=dt, device=dev)
+                ops.paged_attention(q.to(dev), c.kd, c.vd, c.table_d, _i32(lens, dev), _i32(start, dev), out, scale=scale, max_new=max_new, workspace=ws)
+                torch.cuda.synchronize()
+                for b in range(3):
+                    lo, hi = start[b], start[b + 1]
+                    o, A, S, count, V = _attn_ref(q[lo:hi], c.k[b], c.v[b], new[b], 0, scale)
+                    bad = ~((out[lo:hi].cpu().double() - o).abs() <= _attn_limit(o, A, torch.zeros_like(S), count, V, dt, hd))
+                    assert not bool(bad.any()), (sign, max_new, b, int(bad.sum()))
+
+
+@pytest.mark.parametrize("dt", DTS)
 def test_attention_rows_without_keys_and_bad_pages(dev, dt):
     """seq_len below the number of new rows: the first rows see nothing and give zeros.  Pages out of range are not seen, a row whose
     pages are all bad gives zeros; lengths past the table's capacity are cut there."""
