@@ -1018,6 +1018,51 @@ def test_verify_odd_values(dev, split):
     assert out.tolist() == want[0] and n_out.tolist() == want[1]
 
 
+def test_verify_split_graph_replay(dev):
+    """A captured verification whose rows are split over workgroups, replayed with other inputs and eager work in between, refused steps among
+    them: every replay equals the eager call, and the workspace is left ready."""
+    from mars5_tts_amd import _lib as L, ops
+    B, V, rows, width = 4, 20011, [3, 1, 5, 2], 5
+    start = [0, 3, 4, 9, 11]
+    side = torch.cuda.Stream(device=dev)
+    g = torch.Generator().manual_seed(31)
+    fixed = dict(target=torch.zeros(11, V, device=dev), draft=torch.zeros(11, V, device=dev), tokens=torch.zeros(11, dtype=torch.int64, device=dev), row_start=_i32(start, dev),
+                 uniforms=torch.zeros(11, device=dev), noise=torch.ones(B, V, device=dev))
+    seq, state = _i32([9, 8, 7, 6], dev), _i32([0] * L.PST_WORDS, dev)
+    ws = torch.zeros(B * L.DRAFT_WS_BYTES, dtype=torch.uint8, device=dev)
+    outs = [(torch.zeros(B, width, dtype=torch.int64, device=dev), _i32([0] * B, dev), _i32([0] * B, dev)) for _ in range(2)]
+
+    def call(o, work, stream=None):
+        ops.draft_verify(*fixed.values(), o[0], o[1], seq_len=seq, keep_len=o[2], workspace=work, stream=stream, plan_state=state)
+
+    torch.cuda.synchronize()
+    graph = ops.Graph()
+    graph.begin(side.cuda_stream)
+    call(outs[0], ws, side.cuda_stream)
+    graph.end(side.cuda_stream)
+    for i in range(6):
+        target = torch.softmax(torch.randn(11, V, generator=g) * 2, -1)
+        fixed["target"].copy_(target)
+        fixed["draft"].copy_(torch.softmax(torch.randn(11, V, generator=g) * 2, -1))
+        tokens = torch.randint(0, V, (11,), generator=g)
+        tokens[1:] = torch.where(torch.rand(10, generator=g) < 0.8, target.argmax(-1)[:-1], tokens[1:])
+        fixed["tokens"].copy_(tokens)
+        fixed["uniforms"].copy_(torch.rand(11, generator=g))
+        fixed["noise"].copy_(torch.empty(B, V).exponential_(generator=g))
+        state[L.PST_STATUS] = 3 if i == 2 else 0
+        for o in outs:
+            o[2].fill_(50 + i)
+        torch.cuda.synchronize()
+        graph.launch(side.cuda_stream)
+        side.synchronize()
+        call(outs[1], None)
+        torch.cuda.synchronize()
+        for a, b in zip(*outs):
+            assert torch.equal(a, b), i
+        assert (outs[0][2].tolist() == [52] * B and bool((outs[0][0] == -1).all())) if i == 2 else int(outs[0][1].min()) >= 1
+        assert not bool(ws.any())
+
+
 def test_verify_keeps_the_targets_distribution(dev):
     """The first token that comes out of a drafted step is distributed as the target, whatever the draft: 20000 requests over 5 tokens, counts
     within 5 standard deviations."""
