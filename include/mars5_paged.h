@@ -9,10 +9,11 @@
 /* ------------------------------------------------------------------------------------
  * Paged serving: a KV cache in blocks that many requests share, several new tokens per request and step (prompt chunks, drafted
  * tokens), n_heads / n_kv_heads query heads per kv head.  One step = m5_paged_plan, then per layer m5_paged_rope_cache and
- * m5_paged_attention, then m5_draft_verify; its keep_len is the next step's (rejected drafts are rolled back there).  All lengths
- * live in device memory: a step is capturable and needs no host read-back.  Caches: block, head and slot strides in elements,
- * features contiguous; block_size a power of two <= 1024; a block id outside [0, n_blocks) is never dereferenced.  Padding (rows
- * from q_start[n_seq] on) is neither computed nor written.
+ * m5_paged_attention, then m5_draft_verify; its keep_len is the next step's (rejected drafts are rolled back there).  Blocks come
+ * back from a request's end only: those behind a window stay with it until it ends.  All lengths live in device memory: a step is
+ * capturable and needs no host read-back.  Caches: block, head and slot strides in elements, features contiguous; block_size a
+ * power of two <= 1024; a block id outside [0, n_blocks) is never dereferenced.  Padding (rows from q_start[n_seq] on) is neither
+ * computed nor written.
  * ------------------------------------------------------------------------------------ */
 
 /* Block tables, slot map, positions and row offsets of one step, from the requests' lengths, in one launch.
@@ -46,8 +47,8 @@ typedef struct {
  * y = x rsqrt(mean(x^2) + eps) w when q_norm / k_norm (fp32 [head_dim]) are given, then the first 2 n_pairs features are
  * rotated by rope[positions[r]] (fp32 [n_pos][n_pairs][cos, sin]): features (2i, 2i + 1) when interleaved, (i, n_pairs + i)
  * otherwise.  fp32 throughout, rounded once.  q -> q_out, k and v -> slot slot_map[r] of the caches.  A row with a slot or position
- * out of range (padding: -1) is skipped and its q_out row left as it was; slots must be distinct (two rows of one slot: either
- * row's values).  q_out may be the q part of qkv itself.  head_dim 64 or 128; 2 n_pairs <= head_dim, n_pairs % 8 == 0; pointers and strides multiples of 16 bytes. */
+ * out of range (padding: -1) is skipped and its q_out row left as it was; slots must be distinct (two rows of one slot: a mixture of
+ * their values).  q_out may be the q part of qkv itself.  head_dim 64 or 128; 2 n_pairs <= head_dim, n_pairs % 8 == 0; pointers and strides multiples of 16 bytes. */
 typedef struct {
     const void* qkv; int64_t qkv_rs;
     int32_t n_rows, n_heads, n_kv_heads, head_dim;
@@ -62,8 +63,10 @@ typedef struct {
 
 /* Attention of every request's new tokens over its paged cache: query row r of request b (rows q_start[b] .. q_start[b + 1])
  * stands at position p = seq_len[b] - (q_start[b + 1] - r) and sees the keys max(0, p - window + 1) .. p (window 0: from 0 on); query head
- * h reads kv head h / (n_heads / n_kv_heads).  Online softmax in fp32, scores never stored.  A row that sees no key, or only keys whose
- * score is -inf, gets zeros; a NaN among the scores that a row sees makes the row NaN; keys on a block id out of range are not seen.
+ * h reads kv head h / (n_heads / n_kv_heads).  Online softmax in fp32, scores never stored.  16-bit calls round a key's weight to their
+ * type for the product with its value (once; sums in fp32, in bf16 tiles of 128 rows of the rounded weights); fp32 calls round none.
+ * A row that sees no key, or only keys whose score is -inf, gets zeros; a NaN among the scores that a row sees makes the row NaN;
+ * keys on a block id out of range are not seen.
  * Keys past a request's length and pages behind it are never used, whatever they hold; row offsets that do not ascend compute
  * nothing or rows of theirs twice, inside the buffers.  max_new: upper bound of the new tokens of one request (speed only: it
  * selects the tiling).

@@ -162,8 +162,9 @@ __global__ __launch_bounds__(NT) void draft_verify_kernel(M5DraftVerifyArgs p, i
 template <typename T>
 int launch(const M5DraftVerifyArgs& a, hipStream_t s) {
     // A vocabulary is split when there are too few requests to fill the chip: about 1024 workgroups, of 4096 entries at least (2048: 10.7 us
-    // instead of 8.7 at 16 x 50257 in 16 bits; twice or four times the workgroups change nothing).  128 x 128011 in fp32: 41 us, 4.8 TB/s,
-    // a copy's rate; one workgroup per request 455 us.
+    // instead of 8.7 at 16 x 50257 in 16 bits; twice or four times the workgroups change nothing).  128 x 128011 in fp32, 197 MB: 41.5 us, 4.7 TB/s,
+    // a copy's rate, where four inputs take turns; 35 us on one input again and again (it fits the last-level cache); one workgroup per
+    // request 455 us.
     int parts = 1;
     if (a.workspace && a.workspace_bytes / M5_DRAFT_WS_BYTES >= a.n_seq) {
         const int by_size = (a.vocab + 4095) / 4096, by_chip = (1024 + a.n_seq - 1) / a.n_seq;
